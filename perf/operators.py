@@ -300,7 +300,9 @@ def _codes(x, kind):
     most = torch.full((), 127.0 if kind == "q8_0" else 7.0, device="cuda")  # a tensor: torch multiplies by a number's inverse
     d = (b.abs().amax(-1) / most).half()
     q = b / d.float()[..., None]  # in f32, as the block format's rule has it
-    q = torch.where(d[..., None] == 0, torch.zeros_like(q), torch.sign(q) * torch.floor(q.abs() + 0.5))
+    whole = torch.trunc(q)
+    q = whole + torch.sign(q) * ((q - whole).abs() >= 0.5)  # halves away from zero
+    q = torch.where(d[..., None] == 0, torch.zeros_like(q), q)
     if kind == "q8_0":
         return (q.clamp(-127, 127) + 128).to(torch.uint8).flatten(-2), d
     q = (q.clamp(-8, 7) + 8).to(torch.uint8)
