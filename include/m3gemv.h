@@ -57,6 +57,7 @@ extern "C" {
 #define M3G_DTYPE_Q4_K 12u
 #define M3G_DTYPE_Q5_K_AS_Q4_K 13u
 #define M3G_DTYPE_Q6_K 14u
+#define M3G_DTYPE_BF16 30u /* activations of the serving operators below only */
 
 /* Library ABI version (bumped on any signature change). */
 M3G_API int m3g_abi_version(void);
@@ -358,12 +359,144 @@ M3G_API int m3g_vm_ffn_dev(const float* x, uint64_t M, uint64_t D, const uint8_t
 M3G_API int m3g_matvec_greedy_noalloc(const float* x, const uint8_t* raw, uint64_t raw_len, uint32_t dtype,
                                       uint64_t in_dim, uint64_t out_dim, uint32_t* token, void* stream);
 
+/* ---------------------------------------------------------------- serving operators
+ *
+ * The stages of a step that advances several sequences at once, verifies
+ * drafted tokens or scores given ones: rotary positions, a quantised KV cache,
+ * attention of the new tokens over it, and log probabilities.  No counterpart
+ * in the reference, whose forward_one (src/inference.rs:953-1152) advances one
+ * sequence by one token over an f32 cache.  Activations are F32, F16 or BF16
+ * device memory (`dtype` of each call); the last dimension is contiguous, the
+ * other strides are in elements and free (not negative).  Calls hold no state:
+ * any number may run at once on different streams, and all can be captured. */
+
+/* Rotary positions.  Pair i of a head, (x[i], x[i + rot_dim/2]), or (x[2i],
+ * x[2i + 1]) when interleaved, turns by positions[token] * f_i with f_i =
+ * theta^(-2i / rot_dim), scaled by `scaling`; elements from rot_dim on are
+ * copied.  Angles are exact to 2^-50 of a turn at any 32-bit position
+ * (negative ones turn backwards). */
+#define M3G_ROPE_NONE 0u
+#define M3G_ROPE_LINEAR 1u /* f_i / factor */
+#define M3G_ROPE_NTK 2u    /* theta * factor^(rot_dim / (rot_dim - 2)) */
+#define M3G_ROPE_YARN 3u   /* f_i / factor below beta_slow turns over orig_ctx, f_i above beta_fast, a ramp in i between */
+#define M3G_ROPE_LLAMA3 4u /* the same between low_freq and high_freq turns, the ramp in the number of turns */
+typedef struct m3g_rope m3g_rope;
+typedef struct {
+    uint32_t head_dim;    /* even, <= 512 */
+    uint32_t rot_dim;     /* even, 2 .. min(head_dim, 256) */
+    uint32_t interleaved; /* 0 or 1 */
+    uint32_t scaling;     /* M3G_ROPE_* */
+    double theta;         /* > 1 */
+    double factor;        /* >= 1 (1 with M3G_ROPE_NONE) */
+    uint64_t orig_ctx;    /* YARN, LLAMA3: positions the model was trained on */
+    double low_freq, high_freq;   /* LLAMA3 (usually 1 and 4) */
+    double beta_fast, beta_slow;  /* YARN (usually 32 and 1) */
+    double magnitude;     /* factor on the turned pairs; 0: 1, and 0.1 ln(factor) + 1 for YARN */
+} m3g_rope_config;
+typedef struct {
+    const void* x;        /* heads of each token: x + token*x_token_stride + head*x_head_stride */
+    void* y;              /* results; may be x itself (with x's strides), no other overlap */
+    uint32_t heads;
+    int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+} m3g_rope_rows;
+/* Host arithmetic only (no device needed); one plan serves every device and stream. */
+M3G_API int m3g_rope_create(const m3g_rope_config* cfg, m3g_rope** out);
+M3G_API void m3g_rope_destroy(m3g_rope* rope);
+/* Turns q and, unless NULL, k.  inverse != 0 turns by the opposite angles (with
+ * the same magnitude): the gradient of the forward call. */
+M3G_API int m3g_rope_dev(const m3g_rope* rope, uint32_t dtype, const int32_t* positions, uint64_t n_tokens,
+                         const m3g_rope_rows* q, const m3g_rope_rows* k, int inverse, void* stream);
+
+/* Paged KV cache in blocks of 32 values (Q8_0 or Q4_0) over memory of the
+ * caller: `pool`, m3g_kv_bytes() bytes, 16-byte aligned.  Per layer four
+ * planes follow each other: K codes, K scales, V codes, V scales, each
+ * [n_pages][n_kv_heads][page_size] rows of head_dim (Q4_0: head_dim/2) code
+ * bytes, or of head_dim/32 f16 scales.  A Q8_0 code byte c stands for
+ * (c - 128) * d; a Q4_0 row holds the 16-byte nibble groups of its blocks as
+ * GGUF has them (low nibbles the first 16 values), n for (n - 8) * d. */
+typedef struct {
+    uint32_t dtype;       /* M3G_DTYPE_Q8_0 or M3G_DTYPE_Q4_0 */
+    uint32_t n_layers, n_kv_heads;
+    uint32_t head_dim;    /* 64 or 128 */
+    uint32_t page_size;   /* positions per page: a power of two, 16 .. 1024 */
+    uint64_t n_pages;     /* < 2^31 */
+} m3g_kv_layout;
+M3G_API int m3g_kv_bytes(const m3g_kv_layout* layout, uint64_t* out);
+
+/* New tokens of a batch of sequences: sequence s has tokens q_start[s] ..
+ * q_start[s+1]-1 of the call's n_tokens, at positions ctx_len[s], ctx_len[s]+1,
+ * ... of its pages page_table[s * max_pages + position / page_size] (device
+ * memory throughout).  Pages may be shared by sequences that only read them.
+ * The kernels check what they read: a sequence with more than max_tokens new
+ * tokens, longer than max_len positions or than its max_pages pages, or with
+ * starts outside [0, n_tokens], is skipped (its output rows stay as they
+ * were) and sets kStatusBadBatch (16) in the device status word; a page
+ * outside the pool is neither read nor written (its positions read as zeros)
+ * and sets kStatusBadPage (32). */
+typedef struct {
+    const int32_t* q_start;    /* [n_seqs + 1] */
+    const int32_t* ctx_len;    /* [n_seqs] */
+    const int32_t* page_table; /* [n_seqs][max_pages] */
+    uint32_t n_seqs, max_pages;
+    uint32_t n_tokens;         /* rows of the tensors of the call */
+    uint32_t max_tokens;       /* most new tokens of one sequence */
+    uint32_t max_len;          /* most positions of one sequence, new tokens included */
+} m3g_kv_batch;
+typedef struct {
+    void* p;                   /* [n_tokens][heads][head_dim] of `dtype` */
+    int64_t token_stride, head_stride;
+} m3g_rows;
+
+/* Quantises the new tokens' K and V rows into their places, block by block as
+ * m3g_quantize_q8_0 / _q4_0 do; a block that those refuse (a value that is
+ * not finite) or whose scale passes the f16 range reads back as NaN.  Two
+ * tokens of one call never share a place (what they would leave there is
+ * unspecified).  Accepted drafts are moved by writing their rows again. */
+M3G_API int m3g_kv_write_dev(const m3g_kv_layout* layout, void* pool, uint32_t layer, const m3g_kv_batch* batch,
+                             uint32_t dtype, const m3g_rows* k, const m3g_rows* v, void* stream);
+/* The values held at the new tokens' places, rounded once to `dtype`; with
+ * ctx_len 0 and a sequence's whole length as its tokens, all of it. */
+M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint32_t layer, const m3g_kv_batch* batch,
+                            uint32_t dtype, const m3g_rows* k, const m3g_rows* v, void* stream);
+
+/* Attention of the new tokens (already written) over the cache: out = sum_i
+ * p_i V_i, p = softmax(scale * q . K_i) over the positions that the token
+ * sees -- all of its sequence's first ctx_len[s], and new token i of the
+ * sequence where bit i % 32 of mask[token * mask_words + i / 32] is set (a
+ * token that is to see itself has its own bit set; mask_words * 32 >=
+ * max_tokens).  mask NULL: every new token up to and including itself.  A
+ * token that sees nothing gets zeros.  Query head h reads KV head h /
+ * (n_heads / n_kv_heads).  scale 0 means 1 / sqrt(head_dim).  q and out are
+ * [n_tokens][n_heads][head_dim] of `dtype`; `out` may be q itself.  Sums are
+ * f32; products take the cached codes exactly (F32: q and p in two f16 parts).
+ * `workspace`: m3g_tree_attn_workspace() bytes of device memory, 16-byte
+ * aligned, contents free, used by one call at a time. */
+M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* layout, uint32_t n_heads, uint64_t* out);
+M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* layout, const void* pool, uint32_t layer,
+                              const m3g_kv_batch* batch, uint32_t dtype, const m3g_rows* q, uint32_t n_heads,
+                              const uint32_t* mask, uint32_t mask_words, float scale, const m3g_rows* out,
+                              void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, lp = x_t - lse(x), of each row of
+ * logits [rows][vocab]: tokens [rows][n_tokens] -> logprob [rows][n_tokens]
+ * (-inf for an id outside the vocabulary); entropy [rows] of the row's
+ * distribution unless NULL; the n_top (<= 32) most probable ids, ties to the
+ * lowest id, with their log probabilities, [rows][n_top] each.  Logits of
+ * -inf have probability 0.  A row with a NaN, a +inf or nothing above -inf
+ * has no distribution: its numbers are NaN (its ids rank NaN below -inf).
+ * tokens, top_id may be NULL with n_tokens, n_top 0.  Sums are f32. */
+M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t rows, uint64_t vocab,
+                                   int64_t row_stride, const int32_t* tokens, uint32_t n_tokens, float* logprob,
+                                   float* entropy, uint32_t n_top, int32_t* top_id, float* top_logprob,
+                                   void* stream);
+
 /* ---------------------------------------------------------------- diagnostics */
 
 /* Error word the kernels of `device` set when a bounded wait gives up
  * (bit 0: a staged-copy wait timed out; bit 3, value 8: a wait for a counter
- * bumped by another GPU or producer ran out, see "peer_wait_us").  clear != 0
- * resets it.  Synchronises the device. */
+ * bumped by another GPU or producer ran out, see "peer_wait_us"; bits 4 and 5,
+ * values 16 and 32: a serving operator met a batch or page outside its limits).
+ * clear != 0 resets it.  Synchronises the device. */
 M3G_API int m3g_device_status(int device, uint32_t* out, int clear);
 
 /* Number of kernel launches this library has enqueued in this process. */

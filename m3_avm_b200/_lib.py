@@ -33,6 +33,36 @@ class DecoderConfig(ctypes.Structure):
     """m3g_decoder_config."""
     _fields_ = [("n_layers", _u64), ("hidden", _u64), ("ffn", _u64), ("n_heads", _u64), ("n_kv_heads", _u64),
                 ("vocab", _u64), ("max_pos", _u64), ("rope_theta", ctypes.c_float)]
+class RopeConfig(ctypes.Structure):
+    """m3g_rope_config."""
+    _fields_ = [("head_dim", _u32), ("rot_dim", _u32), ("interleaved", _u32), ("scaling", _u32),
+                ("theta", ctypes.c_double), ("factor", ctypes.c_double), ("orig_ctx", _u64),
+                ("low_freq", ctypes.c_double), ("high_freq", ctypes.c_double), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class RopeRows(ctypes.Structure):
+    """m3g_rope_rows."""
+    _fields_ = [("x", _vp), ("y", _vp), ("heads", _u32), ("x_token_stride", ctypes.c_int64),
+                ("x_head_stride", ctypes.c_int64), ("y_token_stride", ctypes.c_int64),
+                ("y_head_stride", ctypes.c_int64)]
+
+
+class KvLayout(ctypes.Structure):
+    """m3g_kv_layout."""
+    _fields_ = [("dtype", _u32), ("n_layers", _u32), ("n_kv_heads", _u32), ("head_dim", _u32), ("page_size", _u32),
+                ("n_pages", _u64)]
+
+
+class KvBatchArgs(ctypes.Structure):
+    """m3g_kv_batch."""
+    _fields_ = [("q_start", _vp), ("ctx_len", _vp), ("page_table", _vp), ("n_seqs", _u32), ("max_pages", _u32),
+                ("n_tokens", _u32), ("max_tokens", _u32), ("max_len", _u32)]
+
+
+class Rows(ctypes.Structure):
+    """m3g_rows."""
+    _fields_ = [("p", _vp), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 # name -> (restype, argtypes); the list every test checks against the header.
@@ -97,6 +127,17 @@ SIGNATURES: dict[str, tuple] = {
     "m3g_vm_matvec_dev": (ctypes.c_int, [_vp, _u64, _u64, _vp, _u64, _u32, _u64, _vp, _vp]),
     "m3g_vm_ffn_dev": (ctypes.c_int, [_vp, _u64, _u64, _vp, _u64, _u32, _u64, _vp, _u64, _u32, _u64, _vp, _u64,
                                       _vp, _u64, _vp, _vp]),
+    "m3g_rope_create": (ctypes.c_int, [ctypes.POINTER(RopeConfig), ctypes.POINTER(_vp)]),
+    "m3g_rope_destroy": (None, [_vp]),
+    "m3g_rope_dev": (ctypes.c_int, [_vp, _u32, _vp, _u64, _vp, _vp, ctypes.c_int, _vp]),
+    "m3g_kv_bytes": (ctypes.c_int, [_vp, ctypes.POINTER(_u64)]),
+    "m3g_kv_write_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
+    "m3g_kv_read_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
+    "m3g_tree_attn_workspace": (ctypes.c_int, [_vp, _u32, ctypes.POINTER(_u64)]),
+    "m3g_tree_attn_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, ctypes.c_float, _vp, _vp,
+                                         _u64, _vp]),
+    "m3g_token_logprobs_dev": (ctypes.c_int, [_u32, _vp, _u64, _u64, ctypes.c_int64, _vp, _u32, _vp, _vp, _u32, _vp,
+                                              _vp, _vp]),
 }
 
 _lib = None

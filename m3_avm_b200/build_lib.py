@@ -52,7 +52,7 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> str:
         return LIB
     gcc = shutil.which("g++") or "/usr/bin/g++"
     cmd = [
-        nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
+        nvcc_path(), *ARCH_FLAGS, "--threads", "0", "-O3", "-lineinfo", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
         "-Xcompiler", "-fvisibility=hidden", "-ccbin", gcc, "-I", INCLUDE, "-I", CSRC,
         "-DM3G_BUILD_LIB", "-o", LIB + ".tmp", *sources(), "-lnccl",
     ]

@@ -706,6 +706,8 @@ bool fused_plannable(int device, uint32_t dtype, long long in_dim, long long row
 unsigned long long peer_wait_ns() { return static_cast<unsigned long long>(g_tune.peer_wait_us) * 1000ull; }
 bool decode_shard_ffn_enabled() { return g_tune.decode_shard_ffn != 0; }
 
+void count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
+
 int status_word(int device, uint32_t** out) {
   DevState* ds = nullptr;
   if (int rc = dev_state(device, &ds)) return rc;

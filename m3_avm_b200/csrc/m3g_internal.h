@@ -11,6 +11,8 @@ enum : uint32_t {
   kStatusBadPos = 2u,       // a decode step found its position outside the KV cache
   kStatusBadToken = 4u,     // a decode step read a token id outside the vocabulary
   kStatusPeerTimeout = 8u,  // a wait for other GPUs' rows gave up
+  kStatusBadBatch = 16u,    // a sequence of a serving batch outside the call's limits (skipped)
+  kStatusBadPage = 32u,     // a page id outside the cache pool (not accessed)
 };
 
 constexpr int kMaxPeers = 8;  // ranks one decoder exchanges rows with (itself included)
@@ -224,6 +226,9 @@ struct Tc8Plan {
 bool plan_tc8(long long in_dim, long long rows, const uint8_t* w, const float* x, int sms, int smem_optin,
               Tc8Plan& p);
 cudaError_t launch_tc8(const Tc8Plan& p, const uint8_t* w, cudaStream_t st, bool pdl);
+
+// Adds to the count of enqueued kernels (m3g_launch_count).
+void count_launches(int n);
 
 int mma_sb_bytes(int fmt);
 cudaError_t launch_gemv_mma(int fmt, const MmaArgs& a, int tps, int wk, int grid, size_t smem, cudaStream_t st,

@@ -1,0 +1,142 @@
+// m3g_serve.cuh -- what the serving operators share: activation types, the
+// planes of the quantised KV cache, and the checked view of a batch.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/m3gemv.h"
+#include "m3g_internal.h"
+
+namespace m3g {
+int host_fail(int code, const char* fmt, ...);
+
+// ---------------------------------------------------------------- activations
+template <class T> struct Act;
+template <> struct Act<float> {
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct Act<__half> {
+  static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+template <> struct Act<__nv_bfloat16> {
+  static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+
+// N consecutive values; VEC: their address is a multiple of 16 bytes (of N * sizeof(T) where that is less).
+template <class T, int N, bool VEC>
+__device__ __forceinline__ void load_act(const T* p, float (&v)[N]) {
+  if constexpr (VEC) {
+    constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16, E = B / sizeof(T);
+    union { uint4 q; uint2 d; T t[E]; } u;
+#pragma unroll
+    for (int i = 0; i < N; i += E) {
+      if constexpr (B == 16) u.q = *reinterpret_cast<const uint4*>(p + i);
+      else u.d = *reinterpret_cast<const uint2*>(p + i);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[i + j] = Act<T>::to(u.t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<T>::to(p[i]);
+  }
+}
+template <class T, int N, bool VEC>
+__device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
+  if constexpr (VEC) {
+    constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16, E = B / sizeof(T);
+    union U { uint4 q; uint2 d; T t[E]; __device__ U() {} } u;
+#pragma unroll
+    for (int i = 0; i < N; i += E) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) u.t[j] = Act<T>::from(v[i + j]);
+      if constexpr (B == 16) *reinterpret_cast<uint4*>(p + i) = u.q;
+      else *reinterpret_cast<uint2*>(p + i) = u.d;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = Act<T>::from(v[i]);
+  }
+}
+
+inline int act_size(uint32_t dtype) {
+  return dtype == M3G_DTYPE_F32 ? 4 : (dtype == M3G_DTYPE_F16 || dtype == M3G_DTYPE_BF16) ? 2 : 0;
+}
+
+// Whether rows of `size`-byte values at p, `strides` apart, all start on 16-byte boundaries.
+inline bool rows_aligned(const void* p, int64_t token_stride, int64_t head_stride, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && token_stride * size % 16 == 0 && head_stride * size % 16 == 0;
+}
+
+// The current device and its status word.
+inline int serve_device(int* dev, uint32_t** status) {
+  if (cudaGetDevice(dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
+  return status_word(*dev, status);
+}
+inline cudaStream_t serve_stream(void* stream) {
+  return stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;
+}
+
+// ---------------------------------------------------------------- the batch
+struct SeqView {
+  int q0, n, ctx;  // first token, new tokens, cached positions; n == 0: nothing to do
+};
+
+// Sequence s of the batch, empty where it passes the call's limits (bad set then).
+__device__ __forceinline__ SeqView seq_view(const m3g_kv_batch& b, long long cap, int s, bool* bad) {
+  const long long q0 = b.q_start[s], q1 = b.q_start[s + 1], ctx = b.ctx_len[s];
+  SeqView v{static_cast<int>(q0), static_cast<int>(q1 - q0), static_cast<int>(ctx)};
+  if (q0 < 0 || q1 < q0 || q1 > b.n_tokens || q1 - q0 > b.max_tokens || ctx < 0 || ctx + (q1 - q0) > cap) {
+    if (!(q0 == q1 && ctx >= 0)) *bad = true;  // no new tokens: nothing is read, whatever the context
+    v.n = 0;
+  }
+  return v;
+}
+
+// Positions a sequence may have: the call's limit and its row of the page table.
+inline __host__ __device__ long long seq_cap(const m3g_kv_batch& b, uint32_t page_size) {
+  const long long rows = static_cast<long long>(b.max_pages) * page_size;
+  return rows < static_cast<long long>(b.max_len) ? rows : static_cast<long long>(b.max_len);
+}
+
+// ---------------------------------------------------------------- the cache
+struct KvPlanes {
+  uint8_t *kc, *ks, *vc, *vs;  // this layer's planes
+  uint32_t* status;
+  int kvh, hd, cb, sb;         // KV heads, head size, code and scale bytes per row
+  int page_shift, page_size;
+  int n_pages;
+};
+
+int kv_check(const m3g_kv_layout* l);
+int kv_batch_check(const m3g_kv_layout* l, const m3g_kv_batch* b);
+// The planes of one layer (checks layout, pool and layer); status: of the current device.
+int kv_planes(const m3g_kv_layout* l, const void* pool, uint32_t layer, KvPlanes* out);
+
+// Row number of (page, head, place) in a plane; a row is cb code or sb scale bytes.
+__device__ __forceinline__ long long kv_row(const KvPlanes& p, int page, int head, int at) {
+  return (static_cast<long long>(page) * p.kvh + head) * p.page_size + at;
+}
+
+template <class Kern, class... Args>
+cudaError_t serve_launch(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e == cudaSuccess) count_launches(1);
+  return e;
+}
+
+}  // namespace m3g

@@ -1,0 +1,44 @@
+"""Log probabilities of given tokens, entropy and the most probable
+alternatives of rows of logits, on CUDA tensors (m3g_token_logprobs_dev)."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+from . import _lib
+from .attention import _OnDevice, _check_ints, _fail, _stream, act_dtype
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: object       # (rows, tokens) f32, None without tokens
+    entropy: object       # (rows,) f32, None unless asked for
+    top_ids: object       # (rows, n_top) int32, None with n_top 0
+    top_logprobs: object  # (rows, n_top) f32, None with n_top 0
+
+
+def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, stream=None) -> TokenLogprobs:
+    """logits (rows, vocab) f32, f16 or bf16 with a contiguous last dimension; tokens int32 (rows, n) ids whose log
+    probabilities are wanted (-inf for an id outside the vocabulary); n_top <= 32 most probable ids of each row."""
+    import torch
+
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _fail("logits: (rows, vocab) with a contiguous last dimension is wanted")
+    if n_top < 0:
+        _fail("n_top must not be negative")
+    rows, vocab = logits.shape
+    n, dev = 0, logits.device
+    lp = ent = ids = tops = None
+    if tokens is not None:
+        n = tokens.shape[-1] if tokens.dim() == 2 else -1
+        _check_ints("tokens", tokens, logits, (rows, n))
+        lp = torch.empty((rows, n), dtype=torch.float32, device=dev)
+    if entropy:
+        ent = torch.empty((rows,), dtype=torch.float32, device=dev)
+    if n_top:
+        ids = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
+        tops = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    with _OnDevice(logits):
+        _lib.check(_lib.load().m3g_token_logprobs_dev(
+            act_dtype(logits), logits.data_ptr(), rows, vocab, logits.stride(0), ptr(tokens), n, ptr(lp), ptr(ent),
+            n_top, ptr(ids), ptr(tops), _stream(logits, stream)))
+    return TokenLogprobs(lp, ent, ids, tops)
