@@ -1,10 +1,38 @@
 // m3g_tree_attn.cu -- attention of drafted tokens over the quantised KV cache.
 //
-// out = softmax(scale * q K^T + mask) V per (token, query head), positions in
-// order with a running maximum and sum.  One CTA per (token, query head); its
-// warps take every fourth position, each lane HD / 32 values of the row, and
-// their partial results join in shared memory.
+// out = softmax(scale * q K^T + mask) V with a running maximum and sum, the
+// cached codes multiplied as they are.
+//
+// Rows.  The query heads that share a KV head and the new tokens of a sequence
+// are the rows of one product (row = token * group + head in group), 16 to a
+// tile; every tile reads its sequence's K and V of one KV head.
+//
+// Products.  mma.sync m16n8k16 in f16 with f32 sums.  A code (c - 128, or
+// n - 8) is an integer that f16 holds exactly: one PRMT puts it behind the
+// exponent of 1024 and one HADD2 takes the offset off.  Scores: 32 products per
+// block, then f32 scores += d * sum, so nothing of K is rounded.  Values: the
+// weight times V's scale, p * d, is the f16 operand and V's codes the exact
+// other one.  q is an exact f16 operand for F16 and BF16 (its rows are scaled by
+// a power of two); for F32 q and p * d are two f16 parts, hi + lo, 22 bits.
+// So that p * d stays in f16's normal range whatever V's scale, d is taken
+// relative to a power of two dref >= every d seen by the warp; when it grows,
+// the sums are rescaled (rare).
+//
+// Work.  Sequences' lengths are only known on the device.  A unit is one
+// (sequence, KV head, row tile), cut into chunks of 128 positions; each CTA adds
+// up all chunks from the lengths and takes an equal, contiguous share, whatever
+// unit borders lie in it.  A unit inside one CTA is written out there; pieces of
+// a cut one go to the workspace, and k_tree_join adds them up in CTA order, so
+// the bits do not depend on timing.  One token of one long sequence is thus
+// spread over all SMs, and a ragged batch is balanced to one chunk.
+//
+// Inside a CTA each of 4 warps owns every fourth group of 32 positions and a
+// ring of stages filled by 16-byte cp.async; it keeps its own maximum, sum and
+// 16 x HD results in registers, so the warps meet only at the end of a piece.
+// The stages are swizzled so that the fragment loads touch all banks.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "m3g_device.cuh"
 #include "m3g_serve.cuh"
@@ -12,93 +40,646 @@
 namespace m3g {
 namespace {
 
+constexpr int kTreeWarps = 4;
+constexpr int kTreeThreads = 32 * kTreeWarps;
+constexpr int kGroup = 32;                      // positions per warp and step
+constexpr int kChunk = kGroup * kTreeWarps;     // positions per unit of work
+constexpr int kTile = 16;                       // rows per tile
+constexpr int kTreeCtasPerSm = 2;
+constexpr int kTreeMaxCtas = 2 * 160;           // CTAs that the workspace is sized for
+
 struct TreeArgs {
   KvPlanes p;
   m3g_kv_batch b;
   m3g_rows q, out;
   const uint32_t* mask;
+  float* parts;  // [2 * CTAs] of a tile's results, then its maxima and sums
+  int4* desc;    // [CTAs] the cut unit that starts in the CTA: sequence (-1: none), KV head, tile, its last CTA
   long long cap;
   int mask_words, n_heads, group;
+  int vec;       // q rows are 16-byte aligned
   float scale;
 };
 
-template <class T, int HD, bool Q8>
-__global__ void __launch_bounds__(128) k_tree_attn(const __grid_constant__ TreeArgs a) {
-  constexpr int DPL = HD / 32;
-  __shared__ float part[4][HD + 2];
-  const int t = blockIdx.x, head = blockIdx.y, kvhead = head / a.group;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int lo = 0, hi = static_cast<int>(a.b.n_seqs);
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.b.q_start[mid] <= t) lo = mid;
-    else hi = mid;
+template <int HD>
+struct Part {
+  static constexpr int kFloats = kTile * HD + 2 * kTile;
+};
+
+__device__ __forceinline__ float tex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Bytes SEL picks of w (two of them), less `off`, as exact f16 values.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t w, __half2 off) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, SEL);  // 1024 + byte
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+__device__ __forceinline__ void cp16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Geometry of a warp's stage: K codes, V codes, K scales, V scales of 32 rows.
+template <int HD, bool Q8>
+struct Stage {
+  static constexpr int CB = Q8 ? HD : HD / 2, SB = HD / 16, NB = HD / 32;
+  static constexpr int CPR = CB / 16;   // 16-byte pieces per row
+  static constexpr int RPL = 128 / CB;  // rows per 128-byte line
+  static constexpr int kCodes = kGroup * CB, kScales = kGroup * SB;
+  static constexpr int kBytes = 2 * (kCodes + kScales);
+  static constexpr int NS = 26112 / kBytes < 8 ? 26112 / kBytes : 8;  // stages: 3 for the largest rows
+  static constexpr int kWarpBytes = NS * kBytes;
+  // Byte offset of 16-byte piece `col` of `row`.  K fragments read one block of
+  // 8 rows at once, V fragments one block of rows 2t (t = 0..3).
+  static __device__ __forceinline__ int k_at(int row, int col) {
+    int slot = (row % RPL) * CPR + col;
+    if (Q8) slot ^= HD == 128 ? (row & 3) << 1 : ((row >> 1) & 1) << 1;
+    else slot ^= HD == 128 ? (row >> 1) & 3 : (row >> 2) & 1;
+    return (row / RPL) * 128 + slot * 16;
   }
-  bool bad = false;
-  const SeqView s = seq_view(a.b, a.cap, lo, &bad);
-  if (bad && threadIdx.x == 0) atomicOr(a.p.status, kStatusBadBatch);
-  if (t < s.q0 || t - s.q0 >= s.n) return;
-  const int j = t - s.q0, len = s.ctx + s.n;
-  const T* q = static_cast<const T*>(a.q.p) + t * a.q.token_stride + head * a.q.head_stride;
-  float qv[DPL], o[DPL], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) {
-    qv[i] = Act<T>::to(q[lane * DPL + i]) * a.scale;
-    o[i] = 0.f;
+  static __device__ __forceinline__ int v_at(int row, int col) {
+    int slot = (row % RPL) * CPR + col;
+    if (Q8) slot ^= ((row >> 1) & 3) << 1;
+    else slot ^= HD == 128 ? (row >> 1) & 3 : (row >> 2) & 1;
+    return (row / RPL) * 128 + slot * 16;
   }
-  auto value = [&](const uint8_t* codes, const uint8_t* scales, long long row, int e) {
-    const float d = __half2float(reinterpret_cast<const __half*>(scales + row * a.p.sb)[e / 32]);
-    if (Q8) return (static_cast<float>(codes[row * a.p.cb + e]) - 128.f) * d;
-    const uint32_t c = codes[row * a.p.cb + e / 32 * 16 + e % 16];
-    return (static_cast<float>(e & 16 ? c >> 4 : c & 15u) - 8.f) * d;
-  };
-  for (int pos = warp; pos < len; pos += 4) {
-    const int i = pos - s.ctx;
-    if (i >= 0 && !(a.mask ? a.mask[static_cast<long long>(t) * a.mask_words + (i >> 5)] >> (i & 31) & 1u : i <= j))
-      continue;
-    const int page = a.b.page_table[static_cast<long long>(lo) * a.b.max_pages + (pos >> a.p.page_shift)];
-    const bool there = page >= 0 && page < a.p.n_pages;
-    if (!there && lane == 0) atomicOr(a.p.status, kStatusBadPage);
-    const long long row = there ? kv_row(a.p, page, kvhead, pos & (a.p.page_size - 1)) : 0;
-    float dot = 0.f;
+};
+
+template <int HD, bool Q8>
+constexpr size_t tree_smem() {
+  const size_t ring = static_cast<size_t>(kTreeWarps) * Stage<HD, Q8>::kWarpBytes;
+  const size_t join = sizeof(float) * kTreeWarps * kTile * (HD + 4 + 2);
+  return ring > join ? ring : join;
+}
+
+__device__ __forceinline__ long long block_sum(long long v, long long* red) {
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) dot += there ? qv[e] * value(a.p.kc, a.p.ks, row, lane * DPL + e) : 0.f;
-    dot = warp_sum(dot);
-    const float mn = fmaxf(m, dot);
-    const float f = m == -INFINITY ? 0.f : expf(m - mn), w = expf(dot - mn);
-    l = l * f + w;
-#pragma unroll
-    for (int e = 0; e < DPL; ++e) o[e] = o[e] * f + (there ? w * value(a.p.vc, a.p.vs, row, lane * DPL + e) : 0.f);
-    m = mn;
-  }
-  if (lane == 0) {
-    part[warp][HD] = m;
-    part[warp][HD + 1] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < DPL; ++e) part[warp][lane * DPL + e] = o[e];
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   __syncthreads();
-  if (threadIdx.x >= HD) return;
-  float M = -INFINITY, L = 0.f, O = 0.f;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, part[w][HD]);
-  for (int w = 0; w < 4; ++w) {
-    if (part[w][HD + 1] == 0.f) continue;
-    const float f = expf(part[w][HD] - M);
-    L += f * part[w][HD + 1];
-    O += f * part[w][threadIdx.x];
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < kTreeWarps; ++w) v += red[w];
+  return v;
+}
+
+// Low n bits set, n clamped to 0 .. 32.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+struct SeqWork {
+  SeqView v;
+  int chunks, tiles;  // chunks per unit, row tiles per KV head
+  __device__ __forceinline__ long long total(int kvh) const {
+    return static_cast<long long>(chunks) * tiles * kvh;
   }
-  static_cast<T*>(a.out.p)[t * a.out.token_stride + head * a.out.head_stride + threadIdx.x] =
-      Act<T>::from(L == 0.f ? 0.f : O / L);
+};
+
+__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool* bad) {
+  SeqWork w;
+  w.v = seq_view(a.b, a.cap, s, bad);
+  w.chunks = w.v.n ? (w.v.ctx + w.v.n + kChunk - 1) / kChunk : 0;
+  w.tiles = static_cast<int>((static_cast<long long>(w.v.n) * a.group + kTile - 1) / kTile);
+  return w;
 }
 
 template <class T, int HD, bool Q8>
-cudaError_t launch_tree(const TreeArgs& a, cudaStream_t st) {
-  return serve_launch(k_tree_attn<T, HD, Q8>, dim3(a.b.n_tokens, a.n_heads), dim3(128), 0, st, false, a);
+__global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(const __grid_constant__ TreeArgs a) {
+  using St = Stage<HD, Q8>;
+  constexpr bool SPLIT = std::is_same<T, float>::value;
+  constexpr int NB = St::NB, NT = kGroup / 8, NO = HD / 8, KS = HD / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long red[kTreeWarps];
+  __shared__ long long found[2];  // the sequence of this CTA's first chunk, its chunks before it
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, t = lane & 3;
+  const int n_seqs = static_cast<int>(a.b.n_seqs), kvh = a.p.kvh;
+
+  // ---------------------------------------------------------------- this CTA's share
+  long long mine = 0;
+  bool bad = false;
+  for (int s = tid; s < n_seqs; s += kTreeThreads) mine += seq_work(a, s, &bad).total(kvh);
+  if (bad && blockIdx.x == 0) atomicOr(a.p.status, kStatusBadBatch);
+  const long long W = block_sum(mine, red);
+  const long long G = gridDim.x < W ? gridDim.x : W;  // CTAs with work
+  if (tid == 0) a.desc[blockIdx.x].x = -1;
+  if (blockIdx.x >= G) return;
+  const long long first = blockIdx.x * W / G, last = (blockIdx.x + 1) * W / G;
+  {
+    long long before = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += kTreeThreads) {
+      const long long own = s0 + tid < n_seqs ? seq_work(a, s0 + tid, &bad).total(kvh) : 0;
+      long long up = own;  // inclusive scan
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xFFFFFFFFu, up, o);
+        if (lane >= o) up += x;
+      }
+      __syncthreads();
+      if (lane == 31) red[warp] = up;
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) up += red[w];
+      const long long begin = before + up - own;
+      if (first >= begin && first < begin + own) {
+        found[0] = s0 + tid;
+        found[1] = begin;
+      }
+      long long all = 0;
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; ++w) all += red[w];
+      before += all;
+      if (first < before) break;  // the same for all threads
+    }
+  }
+  __syncthreads();
+  int seq = static_cast<int>(found[0]);
+  SeqWork sw = seq_work(a, seq, &bad);
+  long long base_chunk = found[1];  // chunks of the sequences before this one
+  long long at = first;             // the next chunk
+
+  uint8_t* ring = smem + warp * St::kWarpBytes;
+  const __half2 off = __half2half2(__ushort_as_half(Q8 ? 0x6480 : 0x6408));  // 1152, 1032
+
+  while (at < last) {
+    while (at >= base_chunk + sw.total(kvh)) {
+      base_chunk += sw.total(kvh);
+      sw = seq_work(a, ++seq, &bad);
+    }
+    const int in_seq = static_cast<int>((at - base_chunk) / sw.chunks);  // unit of the sequence
+    const int c0 = static_cast<int>((at - base_chunk) % sw.chunks);
+    const int c1 = static_cast<int>(min(static_cast<long long>(sw.chunks), c0 + (last - at)));
+    const int head = in_seq / sw.tiles, tile = in_seq % sw.tiles;
+    const int ctx = sw.v.ctx, len = sw.v.ctx + sw.v.n, rows = sw.v.n * a.group;
+    const int32_t* table = a.b.page_table + static_cast<long long>(seq) * a.b.max_pages;
+
+    // ---------------------------------------------------------------- copies
+    int pg[2];  // pages of the next step's two groups of 16 positions
+    auto pages_of = [&](int c) {
+      const int p0 = c * kChunk + warp * kGroup;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) pg[h] = c < c1 && p0 + 16 * h < len ? table[(p0 + 16 * h) >> a.p.page_shift] : 0;
+    };
+    auto issue = [&](int c) {
+      if (c < c1) {
+        const int p0 = c * kChunk + warp * kGroup, valid = min(kGroup, len - p0);
+        uint8_t* st = ring + ((c - c0) % St::NS) * St::kBytes;
+        long long row[2];
+        int have[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool there = pg[h] >= 0 && pg[h] < a.p.n_pages;
+          if (!there && valid > 16 * h && lane == 0) atomicOr(a.p.status, kStatusBadPage);
+          row[h] = there ? kv_row(a.p, pg[h], head, (p0 + 16 * h) & (a.p.page_size - 1)) : 0;
+          have[h] = there ? min(16, valid - 16 * h) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < St::CPR; ++i) {
+          const int x = i * 32 + lane, rw = x / St::CPR, col = x % St::CPR, h = i * 32 / (16 * St::CPR);
+          const long long off16 = row[h] * St::CB + (x % (16 * St::CPR)) * 16;
+          const int bytes = (rw & 15) < have[h] ? 16 : 0;
+          cp16(st + St::k_at(rw, col), a.p.kc + off16, bytes);
+          cp16(st + St::kCodes + St::v_at(rw, col), a.p.vc + off16, bytes);
+        }
+        constexpr int SP = 16 / St::SB, PPG = 16 / SP;  // rows per 16 bytes of scales; pieces per group
+        if (lane < 4 * PPG) {
+          const int v = lane / (2 * PPG), x = lane % (2 * PPG), h = x / PPG, rw = x % PPG * SP;
+          const int bytes = max(0, min(16, (have[h] - rw) * St::SB));
+          const uint8_t* src = (v ? a.p.vs : a.p.ks) + (row[h] + rw) * St::SB;
+          cp16(st + 2 * St::kCodes + v * St::kScales + x * 16, src, bytes);
+        }
+      }
+      cp_commit();
+      pages_of(c + 1);
+    };
+    pages_of(c0);
+#pragma unroll
+    for (int i = 0; i < St::NS - 1; ++i) issue(c0 + i);
+
+    // ---------------------------------------------------------------- q
+    const T* qp[2];
+    int token[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = tile * kTile + r + 8 * i;
+      token[i] = row / a.group;
+      qp[i] = row < rows ? static_cast<const T*>(a.q.p) + (sw.v.q0 + token[i]) * a.q.token_stride +
+                               (head * a.group + row % a.group) * a.q.head_stride
+                         : nullptr;
+      if (row >= rows) token[i] = 0;
+    }
+    uint32_t qh[KS][4], ql[SPLIT ? KS : 1][4];
+    float row_scale[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x[KS][4];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        // the 8 values of block b that this thread's fragments hold
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float (&w)[4] = x[2 * b + s];
+          const int d = Q8 ? 32 * b + 8 * t + 4 * s : 32 * b + 16 * s + 4 * t;
+          if (!qp[i]) w[0] = w[1] = w[2] = w[3] = 0.f;
+          else if (a.vec) load_act<T, 4, true>(qp[i] + d, w);
+          else load_act<T, 4, false>(qp[i] + d, w);
+        }
+      }
+      float most = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[k][e]));
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+      // times a power of two that puts the largest into [2^10, 2^11)
+      const int e = max(11, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
+      const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23);
+      row_scale[i] = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 10) << 23);
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float v0 = x[k][2 * h] * up, v1 = x[k][2 * h + 1] * up;
+          const uint32_t hi = pack_f16(v0, v1);
+          qh[k][2 * h + i] = hi;
+          if (SPLIT) {
+            const float2 f = unpack_f16(hi);
+            ql[k][2 * h + i] = pack_f16(v0 - f.x, v1 - f.y);
+          }
+        }
+    }
+
+    // ---------------------------------------------------------------- the piece's positions
+    float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float dref = 0x1p-24f;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+
+    for (int c = c0; c < c1; ++c) {
+      cp_wait<St::NS - 2>();
+      __syncwarp();
+      issue(c + St::NS - 1);
+      const int p0 = c * kChunk + warp * kGroup;
+      if (p0 >= len) continue;
+      const uint8_t* st = ring + ((c - c0) % St::NS) * St::kBytes;
+      const uint8_t* kcodes = st;
+      const uint8_t* vcodes = st + St::kCodes;
+      const uint8_t* kscales = st + 2 * St::kCodes;
+      const uint8_t* vscales = kscales + St::kScales;
+
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int row = 8 * nt + r;
+        uint32_t dk[NB];  // scales of positions 8nt + 2t and + 1: block pairs of the one, then of the other
+        if (NB == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(kscales + (8 * nt + 2 * t) * St::SB);
+          dk[0] = x.x; dk[1] = x.y; dk[NB - 2] = x.z; dk[NB - 1] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(kscales + (8 * nt + 2 * t) * St::SB);
+          dk[0] = x.x; dk[1] = x.y;
+        }
+        float d0[NB], d1[NB];
+#pragma unroll
+        for (int h = 0; h < NB / 2; ++h) {
+          const float2 x = unpack_f16(dk[h]), y = unpack_f16(dk[NB / 2 + h]);
+          d0[2 * h] = x.x; d0[2 * h + 1] = x.y;
+          d1[2 * h] = y.x; d1[2 * h + 1] = y.y;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          uint32_t w[2];
+          if (Q8) {
+            const uint2 x = *reinterpret_cast<const uint2*>(kcodes + St::k_at(row, 2 * b + (t >> 1)) + (t & 1) * 8);
+            w[0] = x.x;
+            w[1] = x.y;
+          } else {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(kcodes + St::k_at(row, b) + t * 4);
+            w[0] = x & 0x0F0F0F0Fu;
+            w[1] = (x >> 4) & 0x0F0F0F0Fu;
+          }
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t b0 = codes2<0x4140>(w[h], off), b1 = codes2<0x4342>(w[h], off);
+            mma_f16(acc, qh[2 * b + h], b0, b1);
+            if (SPLIT) mma_f16(acc, ql[SPLIT ? 2 * b + h : 0], b0, b1);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float d = e & 1 ? d1[b] : d0[b];
+            s[nt][e] = b ? fmaf(d, acc[e], s[nt][e]) : d * acc[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] *= row_scale[e >> 1];
+      }
+
+      // ------------------------------------------------------------ mask
+      const bool tail = p0 + kGroup > ctx;  // new tokens, or positions behind the sequence
+      if (tail) {
+        uint32_t vis[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int i0 = p0 - ctx;  // the first position as a new token's number
+          if (!a.mask) {
+            vis[i] = low_bits(token[i] + 1 - i0);
+          } else {
+            const uint32_t* mrow = a.mask + static_cast<long long>(sw.v.q0 + token[i]) * a.mask_words;
+            const int wd = i0 >> 5;  // floor: -1 and lower while context positions come first
+            const uint32_t lo = wd >= 0 && wd < a.mask_words ? mrow[wd] : 0u;
+            const uint32_t hi = wd + 1 >= 0 && wd + 1 < a.mask_words ? mrow[wd + 1] : 0u;
+            vis[i] = __funnelshift_r(lo, hi, i0 & 31) | low_bits(-i0);
+          }
+          vis[i] &= low_bits(len - p0);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(vis[e >> 1] >> (8 * nt + 2 * t + (e & 1)) & 1u)) s[nt][e] = -INFINITY;
+      }
+
+      // ------------------------------------------------------------ softmax
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
+      float ref[2], grow[2];
+      bool grew = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
+        const float mn = fmaxf(m[i], top[i]);
+        ref[i] = mn == -INFINITY ? 0.f : mn;
+        grow[i] = tex2(m[i] - ref[i]);
+        grew = grew || mn > m[i];
+        m[i] = mn;
+      }
+      // V's scales: the largest of this step against dref
+      uint32_t dv[NT][NB];
+      __half2 big = __half2half2(__ushort_as_half(0));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (NB == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vscales + (8 * nt + 2 * t) * St::SB);
+          dv[nt][0] = x.x; dv[nt][1] = x.y; dv[nt][NB - 2] = x.z; dv[nt][NB - 1] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(vscales + (8 * nt + 2 * t) * St::SB);
+          dv[nt][0] = x.x; dv[nt][1] = x.y;
+        }
+#pragma unroll
+        for (int h = 0; h < NB; ++h) big = __hmax2(big, *reinterpret_cast<const __half2*>(&dv[nt][h]));
+      }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) big = __hmax2(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
+      const float dmax = fmaxf(__low2float(big), __high2float(big));
+      float shrink = 1.f;
+      if (dmax > dref) {  // the same for all lanes
+        const float up = __uint_as_float((__float_as_uint(dmax) + 0x7FFFFFu) & 0x7F800000u);
+        shrink = dref / up;
+        dref = up;
+      }
+      if (__any_sync(0xFFFFFFFFu, grew) || shrink != 1.f) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] *= grow[e >> 1] * shrink;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) l[i] *= grow[i];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[nt][e] = tex2(s[nt][e] - ref[e >> 1]);
+          l[e >> 1] += s[nt][e];
+        }
+
+      // ------------------------------------------------------------ values
+      const float dinv = 0x1p14f / dref;  // p * d * dinv <= 2^14
+#pragma unroll
+      for (int kk = 0; kk < kGroup / 16; ++kk) {
+        uint32_t vw[NB][4];  // codes of positions 16kk + {2t, 2t + 1, 2t + 8, 2t + 9}, four dims of each block
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = 16 * kk + 2 * t + (k & 1) + 8 * (k >> 1);
+            if (Q8) {
+              vw[b][k] = *reinterpret_cast<const uint32_t*>(vcodes + St::v_at(row, 2 * b + (r >> 2)) + (r & 3) * 4);
+            } else {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(vcodes + St::v_at(row, b) + (r & 3) * 4);
+              vw[b][k] = (x >> (r & 4)) & 0x0F0F0F0Fu;
+            }
+          }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // positions 16kk + 8h + 2t, + 1
+            const int nt = 2 * kk + h;
+            const float2 x = unpack_f16(dv[nt][b / 2]), y = unpack_f16(dv[nt][NB / 2 + b / 2]);
+            const float e0 = (b & 1 ? x.y : x.x) * dinv, e1 = (b & 1 ? y.y : y.x) * dinv;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float w0 = s[nt][2 * i] * e0, w1 = s[nt][2 * i + 1] * e1;
+              if (tail) {  // a position that the row does not see adds nothing, NaN or not
+                w0 = s[nt][2 * i] == 0.f ? 0.f : w0;
+                w1 = s[nt][2 * i + 1] == 0.f ? 0.f : w1;
+              }
+              const uint32_t hi = pack_f16(w0, w1);
+              ph[2 * h + i] = hi;
+              if (SPLIT) {
+                const float2 f = unpack_f16(hi);
+                pl[2 * h + i] = pack_f16(w0 - f.x, w1 - f.y);
+              }
+            }
+          }
+          const uint32_t a01 = __byte_perm(vw[b][0], vw[b][1], 0x5140), a23 = __byte_perm(vw[b][0], vw[b][1], 0x7362);
+          const uint32_t b01 = __byte_perm(vw[b][2], vw[b][3], 0x5140), b23 = __byte_perm(vw[b][2], vw[b][3], 0x7362);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = i < 2 ? a01 : a23, y = i < 2 ? b01 : b23;
+            const uint32_t b0 = i & 1 ? codes2<0x4342>(x, off) : codes2<0x4140>(x, off);
+            const uint32_t b1 = i & 1 ? codes2<0x4342>(y, off) : codes2<0x4140>(y, off);
+            mma_f16(o[4 * b + i], ph, b0, b1);
+            if (SPLIT) mma_f16(o[4 * b + i], pl, b0, b1);
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+
+    // ---------------------------------------------------------------- join the warps
+    constexpr int LD = HD + 4;
+    float* jo = reinterpret_cast<float*>(smem);            // [warps][16][LD]
+    float* jm = jo + kTreeWarps * kTile * LD;              // [warps][16] maxima, then sums
+    float* jl = jm + kTreeWarps * kTile;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
+    }
+    __syncthreads();  // every warp is done with its ring
+    const float back = dref * 0x1p-14f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float* dst = jo + (warp * kTile + r + 8 * i) * LD;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const int n = 2 * t + cc;  // column of the fragment
+          const int d = Q8 ? 32 * b + 4 * n : 32 * b + 4 * (n & 3) + 16 * (n >> 2);
+          const int e = 2 * i + cc;
+          *reinterpret_cast<float4*>(dst + d) = make_float4(o[4 * b][e] * back, o[4 * b + 1][e] * back,
+                                                            o[4 * b + 2][e] * back, o[4 * b + 3][e] * back);
+        }
+      if (t == 0) {
+        jm[warp * kTile + r + 8 * i] = m[i];
+        jl[warp * kTile + r + 8 * i] = l[i];
+      }
+    }
+    __syncthreads();
+    {
+      constexpr int DPT = HD / 8;  // dims per thread, 8 threads to a row
+      const int row = tid >> 3, d0 = (tid & 7) * 4;
+      float M = -INFINITY, L = 0.f, O[DPT], f[kTreeWarps];
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; ++w) M = fmaxf(M, jm[w * kTile + row]);
+      const float rf = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int d = 0; d < DPT; ++d) O[d] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; ++w) {
+        f[w] = tex2(jm[w * kTile + row] - rf);
+        L += f[w] * jl[w * kTile + row];
+#pragma unroll
+        for (int d = 0; d < DPT; d += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(jo + (w * kTile + row) * LD + d0 + 8 * d);
+          O[d] += f[w] * x.x;
+          O[d + 1] += f[w] * x.y;
+          O[d + 2] += f[w] * x.z;
+          O[d + 3] += f[w] * x.w;
+        }
+      }
+      const int grow_row = tile * kTile + row;
+      if (c0 == 0 && c1 == sw.chunks) {
+        if (grow_row < rows) {
+          T* y = static_cast<T*>(a.out.p) + (sw.v.q0 + grow_row / a.group) * a.out.token_stride +
+                 (head * a.group + grow_row % a.group) * a.out.head_stride;
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+          for (int d = 0; d < DPT; d += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[d0 + 8 * d + e] = Act<T>::from(L == 0.f ? 0.f : O[d + e] * inv);
+        }
+      } else {
+        float* part = a.parts + static_cast<long long>(2 * blockIdx.x + (c0 == 0)) * Part<HD>::kFloats;
+#pragma unroll
+        for (int d = 0; d < DPT; d += 4)
+          *reinterpret_cast<float4*>(part + row * HD + d0 + 8 * d) = make_float4(O[d], O[d + 1], O[d + 2], O[d + 3]);
+        if ((tid & 7) == 0) {
+          part[kTile * HD + row] = M;
+          part[kTile * HD + kTile + row] = L;
+        }
+        if (tid == 0 && c0 == 0) {
+          const long long end = base_chunk + static_cast<long long>(in_seq + 1) * sw.chunks;  // the unit's end
+          a.desc[blockIdx.x] = make_int4(seq, head, tile, static_cast<int>((end * G - 1) / W));
+        }
+      }
+    }
+    __syncthreads();  // the join buffer becomes the ring again
+    at += c1 - c0;
+  }
+  grid_dep_launch();
+}
+
+// The pieces of the units that were cut, in CTA order: one CTA per main CTA,
+// one warp per row.
+template <class T, int HD>
+__global__ void __launch_bounds__(32 * kTile) k_tree_join(const __grid_constant__ TreeArgs a) {
+  constexpr int DPL = HD / 32;
+  grid_dep_wait();
+  const int4 u = a.desc[blockIdx.x];
+  if (u.x < 0) return;
+  const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool bad = false;
+  const SeqView s = seq_view(a.b, a.cap, u.x, &bad);
+  const int grow_row = u.z * kTile + row;
+  if (grow_row >= s.n * a.group) return;
+  const int n = u.w - static_cast<int>(blockIdx.x) + 1;  // pieces
+  auto part = [&](int i) {  // this CTA's piece starts the unit, the others continue it
+    return a.parts + static_cast<long long>(i ? 2 * (blockIdx.x + i) : 2 * blockIdx.x + 1) * Part<HD>::kFloats;
+  };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[kTile * HD + row]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float L = 0.f, O[DPL];
+#pragma unroll
+  for (int d = 0; d < DPL; ++d) O[d] = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
+    const float* p = part(i);
+    const float f = tex2(p[kTile * HD + row] - ref);
+    L += f * p[kTile * HD + kTile + row];
+    float v[DPL];
+    load_act<float, DPL, true>(p + row * HD + lane * DPL, v);
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) O[d] += f * v[d];
+  }
+  T* y = static_cast<T*>(a.out.p) + (s.q0 + grow_row / a.group) * a.out.token_stride +
+         (u.y * a.group + grow_row % a.group) * a.out.head_stride;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int d = 0; d < DPL; ++d) y[lane * DPL + d] = Act<T>::from(L == 0.f ? 0.f : O[d] * inv);
+}
+
+template <class T, int HD, bool Q8>
+cudaError_t launch_tree(const TreeArgs& a, int sms, cudaStream_t st) {
+  constexpr size_t smem = tree_smem<HD, Q8>();
+  cudaError_t e = cudaFuncSetAttribute(k_tree_attn<T, HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  const int grid = std::min(kTreeMaxCtas, kTreeCtasPerSm * sms);
+  e = serve_launch(k_tree_attn<T, HD, Q8>, dim3(grid), dim3(kTreeThreads), smem, st, false, a);
+  if (e != cudaSuccess || a.cap <= kChunk) return e;  // one chunk per unit: none is cut
+  return serve_launch(k_tree_join<T, HD>, dim3(grid), dim3(32 * kTile), 0, st, true, a);
 }
 template <class T>
-cudaError_t launch_tree_t(const TreeArgs& a, bool q8, cudaStream_t st) {
-  if (a.p.hd == 64) return q8 ? launch_tree<T, 64, true>(a, st) : launch_tree<T, 64, false>(a, st);
-  return q8 ? launch_tree<T, 128, true>(a, st) : launch_tree<T, 128, false>(a, st);
+cudaError_t launch_tree_t(const TreeArgs& a, bool q8, int sms, cudaStream_t st) {
+  if (a.p.hd == 64) return q8 ? launch_tree<T, 64, true>(a, sms, st) : launch_tree<T, 64, false>(a, sms, st);
+  return q8 ? launch_tree<T, 128, true>(a, sms, st) : launch_tree<T, 128, false>(a, sms, st);
 }
 
 int check_heads(const m3g_kv_layout* l, uint32_t n_heads) {
@@ -117,7 +698,8 @@ M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* l, uint32_t n_heads, ui
   *out = 0;
   if (int rc = m3g::kv_check(l)) return rc;
   if (int rc = m3g::check_heads(l, n_heads)) return rc;
-  *out = 16;
+  const uint64_t part = sizeof(float) * (l->head_dim == 64 ? m3g::Part<64>::kFloats : m3g::Part<128>::kFloats);
+  *out = m3g::kTreeMaxCtas * (sizeof(int4) + 2 * part);
   return M3G_OK;
 }
 
@@ -150,8 +732,13 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
     return host_fail(M3G_EINVAL, "workspace of %llu bytes (16-byte aligned, %llu needed)",
                      static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(need));
-  int dev = 0;
+  int dev = 0, sms = 0;
   if (int rc = serve_device(&dev, &a.p.status)) return rc;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return host_fail(M3G_ECUDA, "device attributes");
+  a.desc = static_cast<int4*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.desc + kTreeMaxCtas);
+  a.vec = rows_aligned(q->p, q->token_stride, q->head_stride, size);
   a.b = *b;
   a.q = *q;
   a.out = *out;
@@ -163,9 +750,9 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(a.p.hd));
   const cudaStream_t st = serve_stream(stream);
   const bool q8 = l->dtype == M3G_DTYPE_Q8_0;
-  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_tree_t<float>(a, q8, st)
-                        : dtype == M3G_DTYPE_F16 ? launch_tree_t<__half>(a, q8, st)
-                                                 : launch_tree_t<__nv_bfloat16>(a, q8, st);
+  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_tree_t<float>(a, q8, sms, st)
+                        : dtype == M3G_DTYPE_F16 ? launch_tree_t<__half>(a, q8, sms, st)
+                                                 : launch_tree_t<__nv_bfloat16>(a, q8, sms, st);
   if (e != cudaSuccess) return host_fail(M3G_ECUDA, "k_tree_attn: %s", cudaGetErrorString(e));
   return M3G_OK;
 }
