@@ -17,72 +17,80 @@ from . import _lib
 
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
 Q4_0, Q8_0 = 2, 8
+
+# torch is imported at the first use: the host-side rules work without it.
+torch = None
 _dtypes: dict = {}
+
+
+def _need_torch():
+    """Binds torch and what each call needs of it (the raw getters cost a tenth of the checked ones)."""
+    global torch, _int32, _current_device, _current_stream
+    import torch as t
+
+    torch, _int32 = t, t.int32
+    _dtypes.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
+    _current_device = getattr(t._C, "_cuda_getDevice", t.cuda.current_device)
+    _current_stream = getattr(t._C, "_cuda_getCurrentRawStream", lambda i: t.cuda.current_stream(i).cuda_stream)
 
 
 def act_dtype(t) -> int:
     """ggml number of an activation tensor's type."""
-    if not _dtypes:
-        import torch
-
-        _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
-    try:
-        return _dtypes[t.dtype]
-    except KeyError:
-        raise _lib.M3GError(_lib.M3G_EINVAL, f"activations of type {t.dtype} (f32, f16 and bf16 are supported)") from None
+    if torch is None:
+        _need_torch()
+    number = _dtypes.get(t.dtype)
+    if number is None:
+        _fail(f"activations of type {t.dtype} (f32, f16 and bf16 are supported)")
+    return number
 
 
-class _OnDevice:
-    """Makes the tensors' device current for a call, where it is not."""
-
-    def __init__(self, t):
-        import torch
-
-        if not t.is_cuda:
-            raise _lib.M3GError(_lib.M3G_EINVAL, "the operators need CUDA tensors")
-        cur = torch.cuda.current_device()
-        self._guard = torch.cuda.device(t.device) if t.device.index != cur else None
-
-    def __enter__(self):
-        if self._guard:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard:
-            self._guard.__exit__(*exc)
+def _device(t) -> int:
+    if torch is None:
+        _need_torch()
+    i = t.get_device()
+    if i < 0:
+        _fail("the operators need CUDA tensors")
+    return i
 
 
-def _stream(t, stream):
-    import torch
-
-    return stream if stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+def _call(fn, device: int, stream, *args) -> None:
+    """fn(*args, stream) with `device` current; stream None: the current one."""
+    if stream is None:
+        stream = _current_stream(device)
+    if device == _current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
 
 
 def _fail(msg):
     raise _lib.M3GError(_lib.M3G_EINVAL, msg)
 
 
-def _check_rows(name, t, like, heads=None, head_dim=None, tokens=None):
-    """t is (tokens, heads, head_dim) with a contiguous last dimension, on like's device."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-        _fail(f"{name}: (tokens, heads, head_dim) with a contiguous last dimension is wanted, got {tuple(t.shape)}")
-    if t.device != like.device:
-        _fail(f"{name} is on {t.device}, not on {like.device}")
-    for what, got, want in (("tokens", t.shape[0], tokens), ("heads", t.shape[1], heads),
-                            ("head_dim", t.shape[2], head_dim)):
-        if want is not None and got != want:
-            _fail(f"{name} has {got} {what}, not {want}")
+def _check_rows(name, t, device=None, heads=None, head_dim=None, tokens=None):
+    """t is (tokens, heads, head_dim) with a contiguous last dimension on `device`; returns its shape and strides."""
+    shape = t.shape
+    if len(shape) != 3:
+        _fail(f"{name}: (tokens, heads, head_dim) is wanted, got {tuple(shape)}")
+    strides = t.stride()
+    if strides[2] != 1 and shape[2] > 1:
+        _fail(f"{name}: the last dimension has to be contiguous")
+    if device is not None and t.get_device() != device:
+        _fail(f"{name} is on {t.device}, not on cuda:{device}")
+    if (tokens is not None and shape[0] != tokens or heads is not None and shape[1] != heads
+            or head_dim is not None and shape[2] != head_dim):
+        _fail(f"{name} is {tuple(shape)}, not ({tokens}, {heads or 'heads'}, {head_dim})")
+    return shape, strides
 
 
-def _check_ints(name, t, like, shape):
-    import torch
-
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape or t.device != like.device:
-        _fail(f"{name}: a contiguous int32 tensor of shape {shape} on {like.device} is wanted")
-
-
-def _rows(t):
-    return _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1))
+def _check_ints(name, t, device, shape):
+    if torch is None:
+        _need_torch()
+    if t.dtype is not _int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.get_device() != device:
+        _fail(f"{name}: a contiguous int32 tensor of shape {shape} on the device of the other tensors is wanted")
 
 
 class Rope:
@@ -104,31 +112,26 @@ class Rope:
     def apply(self, positions, q, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
         """Turns q and k (k may be None) at int32 `positions` (tokens,); q_out, k_out may be q and k themselves.
         inverse: by the opposite angles, the gradient of the forward call."""
-        import torch
-
-        n = positions.numel()
-        _check_ints("positions", positions, q, (n,))
-        _check_rows("q", q, q, head_dim=self.head_dim, tokens=n)
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        pairs = [(q, q_out)]
-        if k is not None:
-            _check_rows("k", k, q, head_dim=self.head_dim, tokens=n)
-            if k_out is None:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            pairs.append((k, k_out))
-        args = []
-        for x, y in pairs:
-            if x.dtype != q.dtype or y.dtype != q.dtype:
+        dtype, n = act_dtype(q), positions.numel()
+        device = _device(q)
+        _check_ints("positions", positions, device, (n,))
+        args, results = [], []
+        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+            if x is None:
+                args.append(None)
+                results.append(None)
+                continue
+            shape, sx = _check_rows(name, x, device, None, self.head_dim, n)
+            if y is None:
+                y = x.new_empty(shape)
+            shape, sy = _check_rows(name + "_out", y, device, shape[1], self.head_dim, n)
+            if x.dtype is not q.dtype or y.dtype is not q.dtype:
                 _fail("q, k and their results have one type")
-            _check_rows("result", y, q, heads=x.shape[1], head_dim=self.head_dim, tokens=n)
-            args.append(_lib.RopeRows(x.data_ptr(), y.data_ptr(), x.shape[1], x.stride(0), x.stride(1), y.stride(0),
-                                      y.stride(1)))
-        with _OnDevice(q):
-            _lib.check(_lib.load().m3g_rope_dev(self._h, act_dtype(q), positions.data_ptr(), n, ctypes.byref(args[0]),
-                                                ctypes.byref(args[1]) if k is not None else None,
-                                                1 if inverse else 0, _stream(q, stream)))
-        return q_out, k_out
+            args.append(_lib.RopeRows(x.data_ptr(), y.data_ptr(), shape[1], sx[0], sx[1], sy[0], sy[1]))
+            results.append(y)
+        _call(_lib.load().m3g_rope_dev, device, stream, self._h, dtype, positions.data_ptr(), n, ctypes.byref(args[0]),
+              ctypes.byref(args[1]) if args[1] is not None else None, 1 if inverse else 0)
+        return results[0], results[1]
 
     def close(self) -> None:
         if getattr(self, "_h", None) and self._h.value:
@@ -149,9 +152,12 @@ class KvBatch:
 
     def __init__(self, q_start, ctx_len, page_table, n_tokens: int, max_tokens: int, max_len: int):
         n = ctx_len.numel()
-        _check_ints("q_start", q_start, q_start, (n + 1,))
-        _check_ints("ctx_len", ctx_len, q_start, (n,))
-        _check_ints("page_table", page_table, q_start, (n, page_table.shape[-1]))
+        self.device = q_start.get_device()
+        _check_ints("q_start", q_start, self.device, (n + 1,))
+        _check_ints("ctx_len", ctx_len, self.device, (n,))
+        if page_table.dim() != 2:
+            _fail("page_table: (sequences, pages) is wanted")
+        _check_ints("page_table", page_table, self.device, (n, page_table.shape[1]))
         if min(n_tokens, max_tokens, max_len) < 0:
             _fail("negative size of the batch")
         self.q_start, self.ctx_len, self.page_table = q_start, ctx_len, page_table
@@ -166,8 +172,8 @@ class KvCache:
 
     def __init__(self, dtype: int, n_layers: int, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int,
                  device: int = 0, pool=None):
-        import torch
-
+        if torch is None:
+            _need_torch()
         if min(n_layers, n_kv_heads, head_dim, page_size, n_pages) < 0:
             _fail("negative size of the cache")
         self.dtype, self.n_layers, self.n_kv_heads, self.head_dim = dtype, n_layers, n_kv_heads, head_dim
@@ -180,19 +186,21 @@ class KvCache:
         elif pool.dtype != torch.uint8 or not pool.is_contiguous() or pool.numel() < need.value:
             _fail(f"the pool: a contiguous uint8 tensor of {need.value} bytes is wanted")
         self.pool = pool
+        self.device = pool.get_device()
         self._workspace_bytes: dict[int, int] = {}
 
     def _io(self, fn, layer, k, v, batch, stream):
-        for name, t in (("k", k), ("v", v)):
-            _check_rows(name, t, self.pool, self.n_kv_heads, self.head_dim, batch.n_tokens)
-        if k.dtype != v.dtype:
+        device, dtype = _device(self.pool), act_dtype(k)
+        if k.dtype is not v.dtype:
             _fail("k and v have one type")
-        if batch.q_start.device != self.pool.device:
+        if batch.device != device:
             _fail("the batch is on another device than the cache")
-        rk, rv = _rows(k), _rows(v)
-        with _OnDevice(self.pool):
-            _lib.check(fn(ctypes.byref(self.layout), self.pool.data_ptr(), layer, ctypes.byref(batch.args),
-                          act_dtype(k), ctypes.byref(rk), ctypes.byref(rv), _stream(self.pool, stream)))
+        rows = []
+        for name, t in (("k", k), ("v", v)):
+            _, strides = _check_rows(name, t, device, self.n_kv_heads, self.head_dim, batch.n_tokens)
+            rows.append(_lib.Rows(t.data_ptr(), strides[0], strides[1]))
+        _call(fn, device, stream, ctypes.byref(self.layout), self.pool.data_ptr(), layer, ctypes.byref(batch.args),
+              dtype, ctypes.byref(rows[0]), ctypes.byref(rows[1]))
 
     def write(self, layer: int, k, v, batch: KvBatch, stream=None) -> None:
         """Quantises the new tokens' rows into their places."""
@@ -200,8 +208,6 @@ class KvCache:
 
     def read(self, layer: int, batch: KvBatch, dtype=None, k_out=None, v_out=None, stream=None):
         """The values held at the new tokens' places, as (k, v) of `dtype` (f32 by default)."""
-        import torch
-
         shape = (batch.n_tokens, self.n_kv_heads, self.head_dim)
         if k_out is None:
             k_out = torch.empty(shape, dtype=dtype or torch.float32, device=self.pool.device)
@@ -226,34 +232,31 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     of word i / 32 says whether the token sees new token i of its sequence; None: all up to and including itself.
     `workspace`: a uint8 tensor of cache.attention_workspace(heads) bytes, used by one call at a time (allocated here
     when None)."""
-    import torch
-
-    _check_rows("q", q, cache.pool, head_dim=cache.head_dim, tokens=batch.n_tokens)
-    heads = q.shape[1]
+    device, dtype = _device(q), act_dtype(q)
+    shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
+    heads = shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_rows("out", out, q, heads, cache.head_dim, batch.n_tokens)
-        if out.dtype != q.dtype:
-            _fail("q and out have one type")
-    if batch.q_start.device != q.device:
+        out = q.new_empty(shape)
+    elif out.dtype is not q.dtype:
+        _fail("q and out have one type")
+    _, so = _check_rows("out", out, device, heads, cache.head_dim, batch.n_tokens)
+    if batch.device != device:
         _fail("the batch is on another device than q")
-    words = 0
+    words, bits = 0, None
     if mask is not None:
         words = mask.shape[-1] if mask.dim() == 2 else 0
-        _check_ints("mask", mask, q, (batch.n_tokens, words))
+        _check_ints("mask", mask, device, (batch.n_tokens, words))
+        bits = mask.data_ptr()
     if scale is not None and not scale > 0:
         _fail("scale must be positive")
-    if stream is not None and workspace is None:
-        _fail("a call on a stream of its own needs its own workspace")
-    with _OnDevice(q):
-        if workspace is None:
-            workspace = torch.empty(cache.attention_workspace(heads), dtype=torch.uint8, device=q.device)
-        elif workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous():
-            _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
-        rq, ro = _rows(q), _rows(out)
-        _lib.check(_lib.load().m3g_tree_attn_dev(
-            ctypes.byref(cache.layout), cache.pool.data_ptr(), layer, ctypes.byref(batch.args), act_dtype(q),
-            ctypes.byref(rq), heads, mask.data_ptr() if mask is not None else None, words, scale or 0.0,
-            ctypes.byref(ro), workspace.data_ptr(), workspace.numel(), _stream(q, stream)))
+    if workspace is None:
+        if stream is not None:
+            _fail("a call on a stream of its own needs its own workspace")
+        workspace = torch.empty(cache.attention_workspace(heads), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
+        _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
+    rq, ro = _lib.Rows(q.data_ptr(), sq[0], sq[1]), _lib.Rows(out.data_ptr(), so[0], so[1])
+    _call(_lib.load().m3g_tree_attn_dev, device, stream, ctypes.byref(cache.layout), cache.pool.data_ptr(), layer,
+          ctypes.byref(batch.args), dtype, ctypes.byref(rq), heads, bits, words, scale or 0.0, ctypes.byref(ro),
+          workspace.data_ptr(), workspace.numel())
     return out

@@ -3,17 +3,21 @@
 //
 // A block is 32 consecutive values of a row: d = f16(max|x| / 127) (Q4_0: 7),
 // code = round(x / d), halves away from zero, clamped -- the rules of
-// quantize_q8_0 / quantize_q4_0 (src/quant.rs:206-264), whose f32 quotient
-// x / d is kept to the bit: the quotient from the reciprocal decides unless it
-// lies within 2^-12 of a border between two codes, where a correctly rounded
-// division does (one value in about 2000).  A block with a value that is not
+// quantize_q8_0 / quantize_q4_0 (src/quant.rs:206-264), whose f32 quotients
+// are kept to the bit.  x times an approximate reciprocal of d is off by 2^-22
+// of the quotient, so it decides unless it lies within 2^-14 (Q4_0: 2^-18) of a
+// border between two codes or d is subnormal in f16 (codes_near_borders then).  max|x| / 127 is a product with the rounded reciprocal and one
+// residual step (Markstein's theorem; equal to the division for every f32).  A block with a value that is not
 // finite, or whose scale passes the f16 range, gets the scale NaN and codes
 // that stand for 0, so that it reads back as NaN.
 //
 // Four threads share a block, 8 values each; a thread's 8 values are one
 // 16-byte load (two for f32) and its codes one 8-byte store.  Both kernels are
-// bound by HBM; a CTA takes kKvTokens tokens, whose places its first threads
-// look up in the page table once.
+// bound by HBM; a CTA takes an even share of the tokens, 64 at a time, whose
+// places its threads look up first, one token each.
+#include <algorithm>
+
+#include "m3g_device.cuh"
 #include "m3g_serve.cuh"
 
 namespace m3g {
@@ -69,7 +73,8 @@ int kv_planes(const m3g_kv_layout* l, const void* pool, uint32_t layer, KvPlanes
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvTokens = 8;  // tokens per CTA
+constexpr int kKvTokens = 64;    // tokens looked up at once
+constexpr int kKvStarts = 1024;  // starts of sequences held in shared memory
 
 struct KvIoArgs {
   KvPlanes p;
@@ -78,148 +83,295 @@ struct KvIoArgs {
   long long cap;
 };
 
-// round(x / d), halves away from zero, of the f32 quotient; inv = 1 / d.
-__device__ __forceinline__ float code_of(float x, float d, float inv) {
-  const float t = fabsf(x) * inv;
-  float q = floorf(t + 0.5f);
-  if (fabsf(t + 0.5f - rintf(t + 0.5f)) < 0x1p-12f) q = roundf(__fdiv_rn(fabsf(x), d));
-  return copysignf(q, x);
+// A thread's 8 codes, in the bytes of two words (two's complement), by the
+// rule.  F32: the quotient of a correctly rounded division.  16-bit values: no
+// quotient but an exact half rounds to one (11-bit numbers: the others are off
+// by 2^-12 at least), so the nearest code is found from the exact residual
+// x - q d; these ties are common (wherever max|x| / 127 is an 11-bit number).
+template <class T>
+__device__ __forceinline__ uint2 codes_near_borders(const float (&v)[8], float d, float inv, float least, float most) {
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float q;
+    if (sizeof(T) == 4) {
+      q = roundf(__fdiv_rn(v[i], d));
+    } else {
+      q = rintf(v[i] * inv);
+      const float e = fmaf(-q, d, v[i]);
+      // away from zero at a tie: where the residual still points away
+      if (e * v[i] > 0.f ? 2.f * fabsf(e) >= d : 2.f * fabsf(e) > d) q += copysignf(1.f, e);
+    }
+    q = d > 0.f ? fminf(fmaxf(q, least), most) : 0.f;
+    w[i >> 2] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xFFu) << (8 * (i & 3));
+  }
+  return make_uint2(w[0], w[1]);
 }
 
-// Places of the CTA's tokens: page * page_size + offset, -1 for none.
-__device__ __forceinline__ void find_places(const KvIoArgs& a, int t0, long long (&place)[kKvTokens]) {
-  const int tid = threadIdx.x;
-  if (tid < kKvTokens) {
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where one is NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Places of the CTA's tokens: page * page_size + offset, -1 for none.  One
+// thread looks up one token, by bisection over the starts of the sequences (in
+// shared memory where they fit).
+__device__ __forceinline__ void find_places(const KvIoArgs& a, int t0, int n_tok, long long* place, int32_t* starts) {
+  const int tid = threadIdx.x, n_seqs = static_cast<int>(a.b.n_seqs);
+  const bool held = n_seqs <= kKvStarts;
+  if (tid < n_tok) {
     const int t = t0 + tid;
-    long long at = -1;
-    if (t < static_cast<int>(a.b.n_tokens)) {
-      int lo = 0, hi = static_cast<int>(a.b.n_seqs);  // the last s with q_start[s] <= t
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.b.q_start[mid] <= t) lo = mid;
-        else hi = mid;
-      }
-      bool bad = false;
-      const SeqView s = seq_view(a.b, a.cap, lo, &bad);
-      if (t >= s.q0 && t - s.q0 < s.n) {
-        const int pos = s.ctx + (t - s.q0);
-        const int page = a.b.page_table[static_cast<long long>(lo) * a.b.max_pages + (pos >> a.p.page_shift)];
-        if (page >= 0 && page < a.p.n_pages)
-          at = kv_row(a.p, page, 0, pos & (a.p.page_size - 1));
-        else
-          atomicOr(a.p.status, kStatusBadPage);
-      }
-      if (bad) atomicOr(a.p.status, kStatusBadBatch);
+    int lo = 0, hi = n_seqs;  // the last s with q_start[s] <= t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((held ? starts[mid] : a.b.q_start[mid]) <= t) lo = mid;
+      else hi = mid;
     }
+    long long at = -1;
+    bool bad = false;
+    const SeqView s = seq_view(a.b, a.cap, lo, &bad);
+    if (t >= s.q0 && t - s.q0 < s.n) {
+      const int pos = s.ctx + (t - s.q0);
+      const int page = a.b.page_table[static_cast<long long>(lo) * a.b.max_pages + (pos >> a.p.page_shift)];
+      if (page >= 0 && page < a.p.n_pages)
+        at = kv_row(a.p, page, 0, pos & (a.p.page_size - 1));
+      else
+        atomicOr(a.p.status, kStatusBadPage);
+    }
+    if (bad) atomicOr(a.p.status, kStatusBadBatch);
     place[tid] = at;
   }
   __syncthreads();
 }
 
-template <class T, bool Q8, bool VEC>
-__global__ void __launch_bounds__(kKvThreads) k_kv_write(const __grid_constant__ KvIoArgs a) {
-  __shared__ long long place[kKvTokens];
-  const int t0 = blockIdx.x * kKvTokens;
-  find_places(a, t0, place);
-  const int octs = a.p.hd / 8;                      // threads per row
-  const int per_token = 2 * a.p.kvh * octs;         // K heads, then V heads
-  const int units = kKvTokens * per_token;          // a multiple of 4: the threads of a block stay together
-  for (int u = threadIdx.x; u < units; u += kKvThreads) {
-    const int ti = u / per_token, w = u - ti * per_token;
-    const int row = w / octs, oct = w - row * octs;
-    const bool is_v = row >= a.p.kvh;
-    const int head = is_v ? row - a.p.kvh : row;
-    const unsigned quad = 0xFu << (threadIdx.x & 28);
-    if (place[ti] < 0) continue;  // the same for all threads of a block
-    const m3g_rows& r = is_v ? a.v : a.k;
-    const T* src = static_cast<const T*>(r.p) + (t0 + ti) * r.token_stride + head * r.head_stride + oct * 8;
-    float x[8];
-    load_act<T, 8, VEC>(src, x);
-    float most = 0.f;
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = fmaxf(most, fabsf(x[i]));
-      finite = finite && fabsf(x[i]) <= 3.402823466e38f;
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) most = fmaxf(most, __shfl_xor_sync(quad, most, o));
-    finite = (__ballot_sync(quad, finite) & quad) == quad;
-    __half dh = __float2half_rn(__fdiv_rn(most, Q8 ? 127.f : 7.f));
-    const float d = __half2float(dh);
-    const bool ok = finite && d <= 65504.f;
-    if (!ok) dh = __ushort_as_half(0x7FFF);
-    const float inv = ok && d > 0.f ? __frcp_rn(d) : 0.f;
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float q = inv > 0.f ? code_of(x[i], d, inv) : 0.f;
-      q = Q8 ? fminf(fmaxf(q, -127.f), 127.f) + 128.f : fminf(fmaxf(q, -8.f), 7.f) + 8.f;
-      c[i] = static_cast<uint32_t>(q);
-    }
-    const long long at = place[ti] + static_cast<long long>(head) * a.p.page_size;
-    uint8_t* codes = is_v ? a.p.vc : a.p.kc;
-    if (Q8) {
-      const uint32_t w0 = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-      const uint32_t w1 = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-      *reinterpret_cast<uint2*>(codes + at * a.p.cb + oct * 8) = make_uint2(w0, w1);
-    } else {
-      uint32_t w0 = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-      uint32_t w1 = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-      const uint32_t h0 = __shfl_xor_sync(quad, w0, 2), h1 = __shfl_xor_sync(quad, w1, 2);
-      if ((oct & 2) == 0)  // the block's first 16 values are the low nibbles
-        *reinterpret_cast<uint2*>(codes + at * a.p.cb + (oct >> 2) * 16 + (oct & 1) * 8) =
-            make_uint2(w0 | h0 << 4, w1 | h1 << 4);
-    }
-    if ((oct & 3) == 0)
-      reinterpret_cast<__half*>((is_v ? a.p.vs : a.p.ks) + at * a.p.sb)[oct >> 2] = dh;
-  }
+__device__ __forceinline__ void hold_starts(const KvIoArgs& a, int32_t* starts) {
+  const int n_seqs = static_cast<int>(a.b.n_seqs);
+  if (n_seqs <= kKvStarts)
+    for (int i = threadIdx.x; i < n_seqs; i += kKvThreads) starts[i] = a.b.q_start[i];
+  __syncthreads();
 }
 
-template <class T, bool Q8, bool VEC>
-__global__ void __launch_bounds__(kKvThreads) k_kv_read(const __grid_constant__ KvIoArgs a) {
-  __shared__ long long place[kKvTokens];
-  const int t0 = blockIdx.x * kKvTokens;
-  find_places(a, t0, place);
-  const int octs = a.p.hd / 8, per_token = 2 * a.p.kvh * octs, units = kKvTokens * per_token;
-  for (int u = threadIdx.x; u < units; u += kKvThreads) {
-    const int ti = u / per_token, w = u - ti * per_token;
-    const int row = w / octs, oct = w - row * octs;
-    const bool is_v = row >= a.p.kvh;
-    const int head = is_v ? row - a.p.kvh : row;
-    if (place[ti] < 0) continue;
-    const long long at = place[ti] + static_cast<long long>(head) * a.p.page_size;
-    const uint8_t* codes = (is_v ? a.p.vc : a.p.kc) + at * a.p.cb;
-    const float d =
-        __half2float(reinterpret_cast<const __half*>((is_v ? a.p.vs : a.p.ks) + at * a.p.sb)[oct >> 2]);
-    float x[8];
-    uint2 q;
-    if (Q8) {
-      q = *reinterpret_cast<const uint2*>(codes + oct * 8);
-    } else {
-      q = *reinterpret_cast<const uint2*>(codes + (oct >> 2) * 16 + (oct & 1) * 8);
-      const int sh = (oct & 2) ? 4 : 0;
-      q.x = q.x >> sh & 0x0F0F0F0Fu;
-      q.y = q.y >> sh & 0x0F0F0F0Fu;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t b = ((i < 4 ? q.x : q.y) >> (8 * (i & 3))) & 0xFFu;
-      x[i] = (static_cast<float>(b) - (Q8 ? 128.f : 8.f)) * d;
-    }
-    const m3g_rows& r = is_v ? a.v : a.k;
-    store_act<T, 8, VEC>(static_cast<T*>(r.p) + (t0 + ti) * r.token_stride + head * r.head_stride + oct * 8, x);
+// How a CTA's threads share the 8-value pieces of its tokens: thread -> one
+// piece of a token (K heads, then V heads) and every `ny`-th token; tokens
+// with more pieces than threads (not FITS) are walked piece by piece.
+template <bool FITS>
+struct KvShare {
+  int octs, per, ny, y0, w0;
+  __device__ __forceinline__ explicit KvShare(const KvPlanes& p) {
+    octs = p.hd / 8;
+    per = 2 * p.kvh * octs;  // a multiple of 16: the four threads of a block stay together
+    ny = FITS ? kKvThreads / per : 1;
+    y0 = FITS ? static_cast<int>(threadIdx.x) / per : 0;
+    w0 = FITS ? static_cast<int>(threadIdx.x) - y0 * per : static_cast<int>(threadIdx.x);
   }
-}
+};
 
+template <class T, bool VEC>
+struct alignas(VEC ? 16 : sizeof(T)) Oct {
+  T t[8];
+};
+
+// Where a thread's piece of a token goes.
+struct KvPiece {
+  uint8_t *codes, *scales;
+  int64_t stride, offset;  // of the activations: between tokens; of the piece in a token
+  int head, oct;
+  bool is_v;
+  __device__ __forceinline__ KvPiece(const KvIoArgs& a, int octs, int w) {
+    // picked by value: a reference picked at run time would make every access a load from memory
+    const int row = w / octs;
+    oct = w - row * octs;
+    is_v = row >= a.p.kvh;
+    head = is_v ? row - a.p.kvh : row;
+    codes = is_v ? a.p.vc : a.p.kc;
+    scales = is_v ? a.p.vs : a.p.ks;
+    stride = is_v ? a.v.token_stride : a.k.token_stride;
+    offset = head * (is_v ? a.v.head_stride : a.k.head_stride) + oct * 8;
+  }
+};
+
+// Codes of 8 values (the four threads of `quad` hold their block) into their place.
 template <class T, bool Q8>
-cudaError_t launch_kv(const KvIoArgs& a, bool vec, bool write, cudaStream_t st) {
-  const dim3 grid((a.b.n_tokens + kKvTokens - 1) / kKvTokens), block(kKvThreads);
+__device__ __forceinline__ void write_piece(const KvPlanes& p, const KvPiece& w, long long place, const T (&x)[8],
+                                            unsigned quad) {
+  float v[8], most = 0.f;
+  unpack_act<T, 8>(x, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max_nan(most, fabsf(v[i]));
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) most = max_nan(most, __shfl_xor_sync(quad, most, o));
+  constexpr float kMost = Q8 ? 127.f : 7.f, kInv = 1.f / kMost;
+  const float q0 = most * kInv;
+  __half dh = __float2half_rn(fmaf(fmaf(-kMost, q0, most), kInv, q0));
+  const float d = __half2float(dh);
+  const bool ok = d <= 65504.f;  // else a value that is not finite, or a scale past the f16 range
+  if (!ok) dh = __ushort_as_half(0x7FFF);
+  // nearest integers by the sum with 1.5 * 2^23; at |x / d| <= 127 (1 + 2^-11) none needs a clamp
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+  bool near = d < 0x1p-14f;
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = v[i] * inv, u = t + 12582912.f;
+    near |= fabsf(t - (u - 12582912.f)) > 0.5f - (Q8 ? 0x1p-14f : 0x1p-18f);
+    c[i] = __float_as_uint(u);
+  }
+  uint32_t w0 = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  uint32_t w1 = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+  if (near) {
+    const uint2 e = codes_near_borders<T>(v, ok ? d : 0.f, inv, Q8 ? -127.f : -8.f, Q8 ? 127.f : 7.f);
+    w0 = e.x;
+    w1 = e.y;
+  }
+  if (!ok) w0 = w1 = 0u;
+  const long long at = place + static_cast<long long>(w.head) * p.page_size;
+  if (Q8) {
+    *reinterpret_cast<uint2*>(w.codes + at * p.cb + w.oct * 8) = make_uint2(w0 ^ 0x80808080u, w1 ^ 0x80808080u);
+  } else {
+    w0 = (w0 & 0x0F0F0F0Fu) ^ 0x08080808u;
+    w1 = (w1 & 0x0F0F0F0Fu) ^ 0x08080808u;
+    const uint32_t g0 = __shfl_xor_sync(quad, w0, 2), g1 = __shfl_xor_sync(quad, w1, 2);
+    if ((w.oct & 2) == 0)  // the block's first 16 values are the low nibbles
+      *reinterpret_cast<uint2*>(w.codes + at * p.cb + (w.oct >> 2) * 16 + (w.oct & 1) * 8) =
+          make_uint2(w0 | g0 << 4, w1 | g1 << 4);
+  }
+  if ((w.oct & 3) == 0) reinterpret_cast<__half*>(w.scales + at * p.sb)[w.oct >> 2] = dh;
+}
+
+// RING (a thread has one piece of a token, 16-byte aligned): its pieces of the
+// next tokens come by cp.async into its own places in shared memory, 128 bytes
+// a thread in flight.
+template <class T, bool Q8, bool VEC, bool FITS>
+__global__ void __launch_bounds__(kKvThreads, 4) k_kv_write(const __grid_constant__ KvIoArgs a) {
+  constexpr bool RING = VEC && FITS;
+  constexpr int PB = 8 * sizeof(T), D = 128 / PB;  // bytes of a piece; pieces in flight
+  __shared__ long long place[kKvTokens];
+  __shared__ int32_t starts[kKvStarts];
+  __shared__ __align__(16) uint8_t ring[RING ? kKvThreads * 128 : 16];
+  const int tid = threadIdx.x;
+  const int t_begin = static_cast<int>(static_cast<long long>(blockIdx.x) * a.b.n_tokens / gridDim.x);
+  const int t_end = static_cast<int>((blockIdx.x + 1ll) * a.b.n_tokens / gridDim.x);
+  const unsigned quad = 0xFu << (tid & 28);
+  const KvShare<FITS> sh(a.p);
+  const bool active = sh.y0 < sh.ny && sh.w0 < sh.per;
+  const KvPiece mine(a, sh.octs, active ? sh.w0 : 0);
+  const T* from = static_cast<const T*>(mine.is_v ? a.v.p : a.k.p) + mine.offset;
+  auto slot = [&](int d, int h) { return ring + ((d * (PB / 16) + h) * kKvThreads + tid) * 16; };
+  auto fetch = [&](int t, int d) {
+    if (active && t < t_end) {
+#pragma unroll
+      for (int h = 0; h < PB / 16; ++h) cp16(slot(d, h), from + t * mine.stride + h * (16 / sizeof(T)), 16);
+    }
+    cp_commit();
+  };
+  if (RING) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) fetch(t_begin + sh.y0 + d * sh.ny, d);
+  }
+  int depth = 0;
+  hold_starts(a, starts);
+  const int batch = kKvTokens / sh.ny * sh.ny;  // a thread's tokens are ny apart across batches too
+  for (int t0 = t_begin; t0 < t_end; t0 += batch) {
+    const int n_tok = min(batch, t_end - t0);
+    find_places(a, t0, n_tok, place, starts);
+    if constexpr (RING) {
+      for (int ti = sh.y0; active && ti < n_tok; ti += sh.ny) {
+        cp_wait<D - 1>();
+        alignas(16) T x[8];
+#pragma unroll
+        for (int h = 0; h < PB / 16; ++h)
+          reinterpret_cast<uint4*>(x)[h] = *reinterpret_cast<const uint4*>(slot(depth, h));
+        fetch(t0 + ti + D * sh.ny, depth);
+        depth = depth + 1 == D ? 0 : depth + 1;
+        if (place[ti] >= 0) write_piece<T, Q8>(a.p, mine, place[ti], x, quad);  // the same for the threads of a block
+      }
+    } else {
+      for (int w = active ? sh.w0 : sh.per; w < sh.per; w += FITS ? sh.per : kKvThreads) {
+        const KvPiece piece(a, sh.octs, w);
+        const T* src = static_cast<const T*>(piece.is_v ? a.v.p : a.k.p) + t0 * piece.stride + piece.offset;
+        for (int ti = sh.y0; ti < n_tok; ti += sh.ny) {
+          if (place[ti] < 0) continue;
+          const Oct<T, VEC> x = *reinterpret_cast<const Oct<T, VEC>*>(src + ti * piece.stride);
+          write_piece<T, Q8>(a.p, piece, place[ti], x.t, quad);
+        }
+      }
+    }
+    __syncthreads();  // the places are read
+  }
+}
+
+template <class T, bool Q8, bool VEC, bool FITS>
+__global__ void __launch_bounds__(kKvThreads, 4) k_kv_read(const __grid_constant__ KvIoArgs a) {
+  __shared__ long long place[kKvTokens];
+  __shared__ int32_t starts[kKvStarts];
+  const int t_begin = static_cast<int>(static_cast<long long>(blockIdx.x) * a.b.n_tokens / gridDim.x);
+  const int t_end = static_cast<int>((blockIdx.x + 1ll) * a.b.n_tokens / gridDim.x);
+  constexpr int U = 8;  // tokens in flight
+  const KvShare<FITS> sh(a.p);
+  hold_starts(a, starts);
+  for (int t0 = t_begin; t0 < t_end; t0 += kKvTokens) {
+    const int n_tok = min(kKvTokens, t_end - t0);
+    find_places(a, t0, n_tok, place, starts);
+    for (int w = sh.y0 < sh.ny ? sh.w0 : sh.per; w < sh.per; w += FITS ? sh.per : kKvThreads) {
+      const KvPiece piece(a, sh.octs, w);
+      const uint8_t* codes = piece.codes + (Q8 ? piece.oct * 8 : (piece.oct >> 2) * 16 + (piece.oct & 1) * 8);
+      const uint8_t* scales = piece.scales + (piece.oct >> 2) * 2;
+      const int down = (piece.oct & 2) ? 4 : 0;
+      T* dst = static_cast<T*>(piece.is_v ? a.v.p : a.k.p) + t0 * piece.stride + piece.offset;
+      for (int ti0 = sh.y0; ti0 < n_tok; ti0 += U * sh.ny) {
+        uint2 q[U];
+        __half d[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int ti = ti0 + k * sh.ny;
+          if (ti < n_tok && place[ti] >= 0) {
+            const long long at = place[ti] + static_cast<long long>(piece.head) * a.p.page_size;
+            q[k] = *reinterpret_cast<const uint2*>(codes + at * a.p.cb);
+            d[k] = *reinterpret_cast<const __half*>(scales + at * a.p.sb);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int ti = ti0 + k * sh.ny;
+          if (ti >= n_tok || place[ti] < 0) continue;
+          if (!Q8) {
+            q[k].x = q[k].x >> down & 0x0F0F0F0Fu;
+            q[k].y = q[k].y >> down & 0x0F0F0F0Fu;
+          }
+          const float f = __half2float(d[k]);
+          Oct<T, VEC> y;
+          float v[8];
+          v[0] = byte_2p23<0>(q[k].x); v[1] = byte_2p23<1>(q[k].x);
+          v[2] = byte_2p23<2>(q[k].x); v[3] = byte_2p23<3>(q[k].x);
+          v[4] = byte_2p23<0>(q[k].y); v[5] = byte_2p23<1>(q[k].y);
+          v[6] = byte_2p23<2>(q[k].y); v[7] = byte_2p23<3>(q[k].y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = (v[i] - (k2p23 + (Q8 ? 128.f : 8.f))) * f;
+          pack_act<T, 8>(y.t, v);
+          *reinterpret_cast<Oct<T, VEC>*>(dst + ti * piece.stride) = y;
+        }
+      }
+    }
+    __syncthreads();  // the places are read
+  }
+}
+
+template <class T, bool Q8, bool VEC>
+cudaError_t launch_kv(const KvIoArgs& a, bool write, int sms, cudaStream_t st) {
+  const dim3 grid(std::min<uint32_t>(a.b.n_tokens, 4u * static_cast<uint32_t>(sms))), block(kKvThreads);
+  const bool fits = 2 * a.p.kvh * (a.p.hd / 8) <= kKvThreads;
   if (write)
-    return vec ? serve_launch(k_kv_write<T, Q8, true>, grid, block, 0, st, false, a)
-               : serve_launch(k_kv_write<T, Q8, false>, grid, block, 0, st, false, a);
-  return vec ? serve_launch(k_kv_read<T, Q8, true>, grid, block, 0, st, false, a)
-             : serve_launch(k_kv_read<T, Q8, false>, grid, block, 0, st, false, a);
+    return fits ? serve_launch(k_kv_write<T, Q8, VEC, true>, grid, block, 0, st, false, a)
+                : serve_launch(k_kv_write<T, Q8, VEC, false>, grid, block, 0, st, false, a);
+  return fits ? serve_launch(k_kv_read<T, Q8, VEC, true>, grid, block, 0, st, false, a)
+              : serve_launch(k_kv_read<T, Q8, VEC, false>, grid, block, 0, st, false, a);
+}
+template <class T>
+cudaError_t launch_kv_t(const KvIoArgs& a, bool q8, bool vec, bool write, int sms, cudaStream_t st) {
+  if (q8) return vec ? launch_kv<T, true, true>(a, write, sms, st) : launch_kv<T, true, false>(a, write, sms, st);
+  return vec ? launch_kv<T, false, true>(a, write, sms, st) : launch_kv<T, false, false>(a, write, sms, st);
 }
 
 int kv_io(const m3g_kv_layout* l, const void* pool, uint32_t layer, const m3g_kv_batch* b, uint32_t dtype,
@@ -239,18 +391,19 @@ int kv_io(const m3g_kv_layout* l, const void* pool, uint32_t layer, const m3g_kv
     vec = vec && rows_aligned(r->p, r->token_stride, r->head_stride, size);
   }
   if (!b->n_tokens || !b->n_seqs) return M3G_OK;
-  int dev = 0;
+  int dev = 0, sms = 0;
   if (int rc = serve_device(&dev, &a.p.status)) return rc;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return host_fail(M3G_ECUDA, "device attributes");
   a.b = *b;
   a.k = *k;
   a.v = *v;
   a.cap = seq_cap(*b, l->page_size);
   const cudaStream_t st = serve_stream(stream);
   const bool q8 = l->dtype == M3G_DTYPE_Q8_0;
-  cudaError_t e;
-  if (dtype == M3G_DTYPE_F32) e = q8 ? launch_kv<float, true>(a, vec, write, st) : launch_kv<float, false>(a, vec, write, st);
-  else if (dtype == M3G_DTYPE_F16) e = q8 ? launch_kv<__half, true>(a, vec, write, st) : launch_kv<__half, false>(a, vec, write, st);
-  else e = q8 ? launch_kv<__nv_bfloat16, true>(a, vec, write, st) : launch_kv<__nv_bfloat16, false>(a, vec, write, st);
+  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_kv_t<float>(a, q8, vec, write, sms, st)
+                        : dtype == M3G_DTYPE_F16 ? launch_kv_t<__half>(a, q8, vec, write, sms, st)
+                                                 : launch_kv_t<__nv_bfloat16>(a, q8, vec, write, sms, st);
   if (e != cudaSuccess) return host_fail(M3G_ECUDA, "%s: %s", write ? "k_kv_write" : "k_kv_read", cudaGetErrorString(e));
   return M3G_OK;
 }

@@ -7,9 +7,13 @@
 // 0.06 rad at position 10^6).  sincospif of the top 32 bits gives cos and sin
 // once per token; all its heads share them through shared memory.
 //
-// Bound: HBM (each element read and written once).  One CTA per token; each
-// thread loads its first units before the angles are ready, so the angle
-// arithmetic hides behind the loads.
+// Bound: HBM (each element read and written once).  A CTA takes a run of tokens.
+// Each thread copies its own pieces of the next kRopeDepth tokens into its own
+// places in shared memory (cp.async; nobody else reads them, so no barrier), so
+// that 3 x 64 bytes a thread are in flight without registers; the angles of as many tokens as there
+// are threads for (one thread per pair) are worked out together, between two
+// barriers, since that chain of some 1000 cycles is what a token waits for.
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -24,12 +28,16 @@ struct m3g_rope {
 namespace m3g {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 512;  // at most; a token takes as few as hold it in U units a thread
+constexpr int kRopeDepth = 3;
+constexpr int rope_units(bool inter) { return inter ? 4 : 2; }  // U: four vectors either way
 constexpr int kMaxPairs = 128;
 
 struct RopeArgs {
   const int32_t* positions;
   m3g_rope_rows r[2];
+  long long n_tokens;
+  int batch;             // tokens whose angles are worked out together
   int heads, heads0;     // rows of both tensors; of the first
   int head_dim, rot;
   int inverse;
@@ -37,110 +45,204 @@ struct RopeArgs {
   unsigned long long turn[kMaxPairs];
 };
 
-// A unit is V pairs (two vectors of V values for the half layout, one of 2V
-// when interleaved) or, behind rot, one vector of V (2V) values to copy.
-template <class T, int V, bool VEC, bool INTER>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 cs[kMaxPairs];
-  constexpr int U = 4;       // units a thread holds at once
-  constexpr int W = 2 * V;   // values of a unit
-  const int t = blockIdx.x, tid = threadIdx.x, half = a.rot / 2;
-  const int np = half / V, nt = (a.head_dim - a.rot + (INTER ? W : V) - 1) / (INTER ? W : V);
-  const int per = np + nt, units = a.heads * per;
-  const int pos = a.positions[t];
-  float v[U][W];
-  auto place = [&](int u, const T** x, T** y, int* c) {
-    const int h = u / per;
-    *c = u - h * per;
-    const m3g_rope_rows& r = a.r[h >= a.heads0];
-    const long long hh = h >= a.heads0 ? h - a.heads0 : h;
-    *x = static_cast<const T*>(r.x) + t * r.x_token_stride + hh * r.x_head_stride;
-    *y = static_cast<T*>(r.y) + t * r.y_token_stride + hh * r.y_head_stride;
+// A unit is two vectors of a head (half layout) or one (interleaved): V pairs,
+// or, behind rot, values to copy.  A thread keeps its place in the head, ny
+// heads apart; U units of a token are in flight.  What bounds the 16-bit types
+// beside HBM is instructions, so loads and stores are the same for turned and
+// copied units, and a thread that holds all of its token's units (ONCE, the
+// usual case) keeps their addresses.
+template <class T, int V, bool VEC, bool INTER, bool ONCE>
+__global__ void __launch_bounds__(kRopeThreads, 2) k_rope(const __grid_constant__ RopeArgs a) {
+  __shared__ float2 cs[2][kRopeThreads];
+  constexpr int U = INTER ? 4 : 2;
+  constexpr int S = INTER ? 2 * V : V;  // values of one vector
+  struct alignas(VEC ? 16 : sizeof(T)) Vec { T t[S]; };
+  const int tid = threadIdx.x, threads = blockDim.x, half = a.rot / 2;
+  const int np = half / V, nt = (a.head_dim - a.rot + S - 1) / S;  // units of pairs; vectors behind them
+  const int per = np + (INTER ? nt : (nt + 1) / 2);
+  // units of a head over the threads, ny heads at once
+  const bool fits = ONCE || per <= threads;
+  const int ny = fits ? threads / per : 1;
+  const int h0 = fits ? tid / per : 0;
+  const int c0 = fits ? tid - h0 * per : tid;
+  const bool active = h0 < ny && c0 < per;
+  // Fields of q's or k's rows picked by value: a reference picked at run time
+  // turns every access to the kernel's arguments into a load from memory.
+  const int64_t xt0 = a.r[0].x_token_stride, xt1 = a.r[1].x_token_stride, xh0 = a.r[0].x_head_stride,
+                xh1 = a.r[1].x_head_stride, yt0 = a.r[0].y_token_stride, yt1 = a.r[1].y_token_stride,
+                yh0 = a.r[0].y_head_stride, yh1 = a.r[1].y_head_stride;
+  const T *x0 = static_cast<const T*>(a.r[0].x), *x1 = static_cast<const T*>(a.r[1].x);
+  T *y0 = static_cast<T*>(a.r[0].y), *y1 = static_cast<T*>(a.r[1].y);
+  Vec lo[U], hi[INTER ? 1 : U];
+  float2 turn[V];
+  // where unit c's vectors lie in a head; the second of a half-layout unit may not exist
+  auto lo_at = [&](int c) { return INTER || c < np ? c * S : a.rot + 2 * (c - np) * S; };
+  auto hi_at = [&](int c) { return c < np ? half + c * S : a.rot + (2 * (c - np) + 1) * S; };
+  auto has_hi = [&](int c) { return !INTER && (c < np || 2 * (c - np) + 1 < nt); };
+  auto get = [&](const T* x, int c, int k) {  // x: the head
+    lo[k] = *reinterpret_cast<const Vec*>(x + lo_at(c));
+    if (has_hi(c)) hi[INTER ? 0 : k] = *reinterpret_cast<const Vec*>(x + hi_at(c));
   };
-  auto load = [&](int u, float (&w)[W]) {
-    const T* x;
-    T* y;
-    int c;
-    place(u, &x, &y, &c);
-    if (INTER) {
-      if (c < np) load_act<T, W, VEC>(x + c * W, w);
-      else if (x != y) load_act<T, W, VEC>(x + a.rot + (c - np) * W, w);
-    } else {
-      float (&lo)[V] = *reinterpret_cast<float(*)[V]>(&w[0]);
-      float (&hi)[V] = *reinterpret_cast<float(*)[V]>(&w[V]);
-      if (c < np) {
-        load_act<T, V, VEC>(x + c * V, lo);
-        load_act<T, V, VEC>(x + half + c * V, hi);
-      } else if (x != y) {
-        load_act<T, V, VEC>(x + a.rot + (c - np) * V, lo);
+  auto put = [&](T* y, int c, int k) {
+    if (c < np) {
+      float p[S], q[S];
+      unpack_act<T, S>(lo[k].t, p);
+      if (!INTER) unpack_act<T, S>(hi[INTER ? 0 : k].t, q);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float& f = INTER ? p[2 * i < S ? 2 * i : 0] : p[i];
+        float& g = INTER ? p[2 * i + 1 < S ? 2 * i + 1 : 0] : q[i];
+        const float f0 = f, g0 = g;
+        f = f0 * turn[i].x - g0 * turn[i].y;
+        g = f0 * turn[i].y + g0 * turn[i].x;
+      }
+      pack_act<T, S>(lo[k].t, p);
+      if (!INTER) pack_act<T, S>(hi[INTER ? 0 : k].t, q);
+    }
+    *reinterpret_cast<Vec*>(y + lo_at(c)) = lo[k];
+    if (has_hi(c)) *reinterpret_cast<Vec*>(y + hi_at(c)) = hi[INTER ? 0 : k];
+  };
+  auto from = [&](long long tok, int h) {
+    return h >= a.heads0 ? x1 + tok * xt1 + (h - a.heads0) * xh1 : x0 + tok * xt0 + h * xh0;
+  };
+  auto to = [&](long long tok, int h) {
+    return h >= a.heads0 ? y1 + tok * yt1 + (h - a.heads0) * yh1 : y0 + tok * yt0 + h * yh0;
+  };
+  const long long t_end = (blockIdx.x + 1) * a.n_tokens / gridDim.x;
+  long long tok = blockIdx.x * a.n_tokens / gridDim.x;
+  constexpr bool RING = ONCE && VEC;
+  extern __shared__ __align__(16) uint8_t ring[];  // [depth][4][threads] vectors, each thread's its own
+  const T* px[U];  // this thread's heads, where it has them at once: of the next token to copy
+  T* py[U];        // of the token at hand
+  auto slot = [&](int d, int v) { return reinterpret_cast<Vec*>(ring + ((d * 4 + v) * threads + tid) * 16); };
+  auto fetch = [&](long long t, int d) {  // the thread's units of token t
+    if (active && t < t_end) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int h = h0 + k * ny;
+        if (h >= a.heads) break;
+        cp16(slot(d, INTER ? k : 2 * k), px[k] + lo_at(c0), 16);
+        if (has_hi(c0)) cp16(slot(d, INTER ? k : 2 * k + 1), px[k] + hi_at(c0), 16);
+        px[k] += h >= a.heads0 ? xt1 : xt0;
       }
     }
+    cp_commit();
   };
-  auto finish = [&](int u, float (&w)[W]) {
-    const T* x;
-    T* y;
-    int c;
-    place(u, &x, &y, &c);
-    if (c >= np) {
-      if (x == y) return;
-      if (INTER) {
-        store_act<T, W, VEC>(y + a.rot + (c - np) * W, w);
-      } else {
-        store_act<T, V, VEC>(y + a.rot + (c - np) * V, *reinterpret_cast<float(*)[V]>(&w[0]));
+  if (ONCE && active) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (h0 + k * ny < a.heads) {
+        px[k] = from(tok, h0 + k * ny);
+        py[k] = to(tok, h0 + k * ny);
+        if (!RING) get(px[k], c0, k);
       }
-      return;
-    }
+  }
+  if (RING) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float& p = w[INTER ? 2 * i : i];
-      float& q = w[INTER ? 2 * i + 1 : V + i];
-      const float2 r = cs[c * V + i];
-      const float p0 = p, q0 = q;
-      p = p0 * r.x - q0 * r.y;
-      q = p0 * r.y + q0 * r.x;
-    }
-    if (INTER) {
-      store_act<T, W, VEC>(y + c * W, w);
-    } else {
-      store_act<T, V, VEC>(y + c * V, *reinterpret_cast<float(*)[V]>(&w[0]));
-      store_act<T, V, VEC>(y + half + c * V, *reinterpret_cast<float(*)[V]>(&w[V]));
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < U; ++k)
-    if (tid + k * kRopeThreads < units) load(tid + k * kRopeThreads, v[k]);
-  if (tid < half) {
+    for (int d = 0; d < kRopeDepth; ++d) fetch(tok + d, d);
+  }
+  int depth = 0;
+  const int my_token = tid / half, my_pair = tid - my_token * half;  // angle of this thread
+  const unsigned long long my_turn = my_token < a.batch ? a.turn[my_pair] : 0;
+  auto angle = [&](int pos, unsigned long long per_position) {
     const long long p = a.inverse ? -static_cast<long long>(pos) : static_cast<long long>(pos);
-    const unsigned long long turns = static_cast<unsigned long long>(p) * a.turn[tid];
+    const unsigned long long turns = static_cast<unsigned long long>(p) * per_position;
     float s, c;
     // the top 32 bits as a signed fraction of a turn, in half turns
     sincospif(static_cast<float>(static_cast<int>(turns >> 32)) * 0x1p-31f, &s, &c);
-    cs[tid] = make_float2(c * a.magnitude, s * a.magnitude);
-  }
-  __syncthreads();
-  for (int u0 = tid; u0 < units; u0 += U * kRopeThreads) {
-    if (u0 != tid) {
-#pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (u0 + k * kRopeThreads < units) load(u0 + k * kRopeThreads, v[k]);
+    return make_float2(c * a.magnitude, s * a.magnitude);
+  };
+  auto position = [&](long long t) { return my_token < a.batch && t + my_token < t_end ? a.positions[t + my_token] : 0; };
+  int pos = position(tok);
+  for (int buf = 0; tok < t_end; buf ^= 1) {
+    if (my_token < a.batch) cs[buf][tid] = angle(pos, my_turn);
+    if (threads < half)  // more pairs than threads (batch 1)
+      for (int i = tid + threads; i < half; i += threads) cs[buf][i] = angle(a.positions[tok], a.turn[i]);
+    pos = position(tok + a.batch);
+    __syncthreads();  // the readers of two batches ago are done with this buffer
+    const long long b_end = min(t_end, tok + a.batch);
+    if (!active) {
+      tok = b_end;
+      continue;
     }
+    for (int b = 0; tok < b_end; ++tok, ++b) {
+      const float2* turns = cs[buf] + b * half;
+      if constexpr (ONCE) {
+        if (c0 < np) {
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (u0 + k * kRopeThreads < units) finish(u0 + k * kRopeThreads, v[k]);
+          for (int i = 0; i < V; ++i) turn[i] = turns[c0 * V + i];
+        }
+        if (RING) cp_wait<kRopeDepth - 1>();
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const int h = h0 + k * ny;
+          if (h >= a.heads) break;
+          if (RING) {
+            lo[k] = *slot(depth, INTER ? k : 2 * k);
+            if (has_hi(c0)) hi[INTER ? 0 : k] = *slot(depth, INTER ? k : 2 * k + 1);
+          }
+          put(py[k], c0, k);
+          py[k] += h >= a.heads0 ? yt1 : yt0;
+          if (!RING) {
+            px[k] += h >= a.heads0 ? xt1 : xt0;
+            if (tok + 1 < t_end) get(px[k], c0, k);
+          }
+        }
+        if (RING) {
+          fetch(tok + kRopeDepth, depth);
+          depth = depth + 1 == kRopeDepth ? 0 : depth + 1;
+        }
+      } else {
+      for (int c = c0; c < per; c += fits ? per : threads) {
+        if (c < np) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) turn[i] = turns[c * V + i];
+        }
+        for (int h = h0; h < a.heads; h += U * ny) {
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+            if (h + k * ny < a.heads) get(from(tok, h + k * ny), c, k);
+#pragma unroll
+          for (int k = 0; k < U; ++k)
+            if (h + k * ny < a.heads) put(to(tok, h + k * ny), c, k);
+        }
+      }
+      }
+    }
   }
+}
+
+template <class Kern>
+cudaError_t launch_ring(Kern kern, dim3 grid, unsigned threads, cudaStream_t st, const RopeArgs& a) {
+  const size_t smem = static_cast<size_t>(kRopeDepth) * 64 * threads;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRopeDepth * 64 * kRopeThreads);
+  return e == cudaSuccess ? serve_launch(kern, grid, dim3(threads), smem, st, false, a) : e;
 }
 
 template <class T, bool INTER>
-cudaError_t launch_rope_t(const RopeArgs& a, bool vec, unsigned grid, cudaStream_t st) {
+cudaError_t launch_rope_t(RopeArgs a, bool vec, int sms, cudaStream_t st) {
   // 16-byte vectors: V pairs are two of them (half layout), or one (interleaved)
   constexpr int V = INTER ? 8 / sizeof(T) : 16 / sizeof(T);
-  if (vec) return serve_launch(k_rope<T, V, true, INTER>, dim3(grid), dim3(kRopeThreads), 0, st, false, a);
-  return serve_launch(k_rope<T, 1, false, INTER>, dim3(grid), dim3(kRopeThreads), 0, st, false, a);
+  const int v = vec ? V : 1, s = INTER ? 2 * v : v;
+  const long long tail = (a.head_dim - a.rot + s - 1) / s;
+  const long long units = a.rot / 2 / v + (INTER ? tail : (tail + 1) / 2);  // per head
+  const long long want = units * ((a.heads + rope_units(INTER) - 1) / rope_units(INTER));
+  const unsigned threads = static_cast<unsigned>(std::min<long long>(kRopeThreads, (want + 31) / 32 * 32));
+  // as many CTAs as are resident at 64 registers a thread
+  const dim3 grid(static_cast<unsigned>(std::min<long long>(a.n_tokens, static_cast<long long>(sms) * (1024 / threads))));
+  a.batch = static_cast<int>(std::max<long long>(1, std::min<long long>(threads / (a.rot / 2), a.n_tokens / grid.x)));
+  // whether a thread's units are all that it has of a token
+  const bool once = units <= threads && rope_units(INTER) * (threads / units) >= a.heads;
+  if (vec)
+    return once ? launch_ring(k_rope<T, V, true, INTER, true>, grid, threads, st, a)
+                : serve_launch(k_rope<T, V, true, INTER, false>, grid, dim3(threads), 0, st, false, a);
+  return once ? serve_launch(k_rope<T, 1, false, INTER, true>, grid, dim3(threads), 0, st, false, a)
+              : serve_launch(k_rope<T, 1, false, INTER, false>, grid, dim3(threads), 0, st, false, a);
 }
 
 template <class T>
-cudaError_t launch_rope(const RopeArgs& a, bool vec, bool inter, unsigned grid, cudaStream_t st) {
-  return inter ? launch_rope_t<T, true>(a, vec, grid, st) : launch_rope_t<T, false>(a, vec, grid, st);
+cudaError_t launch_rope(const RopeArgs& a, bool vec, bool inter, int sms, cudaStream_t st) {
+  return inter ? launch_rope_t<T, true>(a, vec, sms, st) : launch_rope_t<T, false>(a, vec, sms, st);
 }
 
 }  // namespace
@@ -244,14 +346,16 @@ M3G_API int m3g_rope_dev(const m3g_rope* rope, uint32_t dtype, const int32_t* po
   a.inverse = inverse != 0;
   a.magnitude = rope->magnitude;
   for (int i = 0; i < rot / 2; ++i) a.turn[i] = rope->turn[i];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
+  a.n_tokens = static_cast<long long>(n_tokens);
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return host_fail(M3G_ECUDA, "no CUDA device");
   const cudaStream_t st = m3g::serve_stream(stream);
   const bool inter = rope->cfg.interleaved != 0;
-  const unsigned grid = static_cast<unsigned>(n_tokens);
-  const cudaError_t e = dtype == M3G_DTYPE_F32   ? m3g::launch_rope<float>(a, vec, inter, grid, st)
-                        : dtype == M3G_DTYPE_F16 ? m3g::launch_rope<__half>(a, vec, inter, grid, st)
-                                                 : m3g::launch_rope<__nv_bfloat16>(a, vec, inter, grid, st);
+  const cudaError_t e = dtype == M3G_DTYPE_F32   ? m3g::launch_rope<float>(a, vec, inter, sms, st)
+                        : dtype == M3G_DTYPE_F16 ? m3g::launch_rope<__half>(a, vec, inter, sms, st)
+                                                 : m3g::launch_rope<__nv_bfloat16>(a, vec, inter, sms, st);
   if (e != cudaSuccess) return host_fail(M3G_ECUDA, "k_rope: %s", cudaGetErrorString(e));
   return M3G_OK;
 }

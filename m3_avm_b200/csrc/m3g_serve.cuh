@@ -2,6 +2,7 @@
 // planes of the quantised KV cache, and the checked view of a batch.
 #pragma once
 #include <cstdint>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,6 +27,50 @@ template <> struct Act<__nv_bfloat16> {
   static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
+
+// A vector's values as f32 and back, two 16-bit values to a conversion.
+template <class T, int N>
+__device__ __forceinline__ void unpack_act(const T (&t)[N], float (&v)[N]) {
+  if constexpr (std::is_same<T, __half>::value && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 f = __half22float2(__halves2half2(t[i], t[i + 1]));
+      v[i] = f.x;
+      v[i + 1] = f.y;
+    }
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 f = __bfloat1622float2(__halves2bfloat162(t[i], t[i + 1]));
+      v[i] = f.x;
+      v[i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = Act<T>::to(t[i]);
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void pack_act(T (&t)[N], const float (&v)[N]) {
+  if constexpr (std::is_same<T, __half>::value && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+      t[i] = __low2half(h);
+      t[i + 1] = __high2half(h);
+    }
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+      t[i] = __low2bfloat16(h);
+      t[i + 1] = __high2bfloat16(h);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = Act<T>::from(v[i]);
+  }
+}
 
 // N consecutive values; VEC: their address is a multiple of 16 bytes (of N * sizeof(T) where that is less).
 template <class T, int N, bool VEC>
@@ -62,6 +107,14 @@ __device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
     for (int i = 0; i < N; ++i) p[i] = Act<T>::from(v[i]);
   }
 }
+
+// 16 bytes from global to shared memory without registers, the last 16 - bytes of them zeros.
+__device__ __forceinline__ void cp16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 inline int act_size(uint32_t dtype) {
   return dtype == M3G_DTYPE_F32 ? 4 : (dtype == M3G_DTYPE_F16 || dtype == M3G_DTYPE_BF16) ? 2 : 0;

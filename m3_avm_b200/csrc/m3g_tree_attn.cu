@@ -95,13 +95,6 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-__device__ __forceinline__ void cp16(void* dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Geometry of a warp's stage: K codes, V codes, K scales, V scales of 32 rows.
 template <int HD, bool Q8>
 struct Stage {

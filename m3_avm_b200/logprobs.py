@@ -5,7 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from . import _lib
-from .attention import _OnDevice, _check_ints, _fail, _stream, act_dtype
+from .attention import _call, _check_ints, _device, _fail, act_dtype
 
 
 class TokenLogprobs(NamedTuple):
@@ -25,20 +25,19 @@ def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, s
     if n_top < 0:
         _fail("n_top must not be negative")
     rows, vocab = logits.shape
+    device, dtype = _device(logits), act_dtype(logits)
     n, dev = 0, logits.device
     lp = ent = ids = tops = None
     if tokens is not None:
         n = tokens.shape[-1] if tokens.dim() == 2 else -1
-        _check_ints("tokens", tokens, logits, (rows, n))
-        lp = torch.empty((rows, n), dtype=torch.float32, device=dev)
+        _check_ints("tokens", tokens, device, (rows, n))
+        lp = logits.new_empty((rows, n), dtype=torch.float32)
     if entropy:
-        ent = torch.empty((rows,), dtype=torch.float32, device=dev)
+        ent = logits.new_empty((rows,), dtype=torch.float32)
     if n_top:
-        ids = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
-        tops = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
+        ids = logits.new_empty((rows, n_top), dtype=torch.int32)
+        tops = logits.new_empty((rows, n_top), dtype=torch.float32)
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    with _OnDevice(logits):
-        _lib.check(_lib.load().m3g_token_logprobs_dev(
-            act_dtype(logits), logits.data_ptr(), rows, vocab, logits.stride(0), ptr(tokens), n, ptr(lp), ptr(ent),
-            n_top, ptr(ids), ptr(tops), _stream(logits, stream)))
+    _call(_lib.load().m3g_token_logprobs_dev, device, stream, dtype, logits.data_ptr(), rows, vocab, logits.stride(0),
+          ptr(tokens), n, ptr(lp), ptr(ent), n_top, ptr(ids), ptr(tops))
     return TokenLogprobs(lp, ent, ids, tops)
