@@ -468,10 +468,14 @@ M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint3
  * token that sees nothing gets zeros.  Query head h reads KV head h /
  * (n_heads / n_kv_heads).  scale 0 means 1 / sqrt(head_dim).  q and out are
  * [n_tokens][n_heads][head_dim] of `dtype`; `out` may be q itself.  Sums are
- * f32; products take the cached codes exactly (F32: q and p in two f16 parts).
- * `workspace`: m3g_tree_attn_workspace() bytes of device memory, 16-byte
- * aligned, contents free, used by one call at a time. */
-M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* layout, uint32_t n_heads, uint64_t* out);
+ * f32.  Products take the cached codes exactly and p as f16 (F32: q and p in
+ * two f16 parts); large BF16 calls with more than 48 rows (tokens times query
+ * heads per KV head) take the cached values, F16 ones V's, rounded to f16.
+ * `workspace`: m3g_tree_attn_workspace() bytes (with the call's dtype, n_heads
+ * and max_tokens) of device memory, 16-byte aligned, contents free, used by
+ * one call at a time. */
+M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* layout, uint32_t dtype, uint32_t n_heads,
+                                    uint32_t max_tokens, uint64_t* out);
 M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* layout, const void* pool, uint32_t layer,
                               const m3g_kv_batch* batch, uint32_t dtype, const m3g_rows* q, uint32_t n_heads,
                               const uint32_t* mask, uint32_t mask_words, float scale, const m3g_rows* out,

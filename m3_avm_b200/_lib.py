@@ -133,7 +133,7 @@ SIGNATURES: dict[str, tuple] = {
     "m3g_kv_bytes": (ctypes.c_int, [_vp, ctypes.POINTER(_u64)]),
     "m3g_kv_write_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
     "m3g_kv_read_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _vp, _vp]),
-    "m3g_tree_attn_workspace": (ctypes.c_int, [_vp, _u32, ctypes.POINTER(_u64)]),
+    "m3g_tree_attn_workspace": (ctypes.c_int, [_vp, _u32, _u32, _u32, ctypes.POINTER(_u64)]),
     "m3g_tree_attn_dev": (ctypes.c_int, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, ctypes.c_float, _vp, _vp,
                                          _u64, _vp]),
     "m3g_token_logprobs_dev": (ctypes.c_int, [_u32, _vp, _u64, _u64, ctypes.c_int64, _vp, _u32, _vp, _vp, _u32, _vp,

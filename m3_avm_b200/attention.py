@@ -216,13 +216,16 @@ class KvCache:
         self._io(_lib.load().m3g_kv_read_dev, layer, k_out, v_out, batch, stream)
         return k_out, v_out
 
-    def attention_workspace(self, n_heads: int) -> int:
-        """Bytes of workspace that attention of n_heads query heads needs."""
-        got = self._workspace_bytes.get(n_heads)
+    def attention_workspace(self, n_heads: int, dtype=None, max_tokens: int = 1) -> int:
+        """Bytes of workspace that attention of n_heads query heads of `dtype` (f32 by default) over at most max_tokens
+        new tokens of a sequence needs."""
+        key = (n_heads, _dtypes.get(dtype, 0), max_tokens)
+        got = self._workspace_bytes.get(key)
         if got is None:
             need = ctypes.c_uint64()
-            _lib.check(_lib.load().m3g_tree_attn_workspace(ctypes.byref(self.layout), n_heads, ctypes.byref(need)))
-            got = self._workspace_bytes[n_heads] = need.value
+            _lib.check(_lib.load().m3g_tree_attn_workspace(ctypes.byref(self.layout), key[1], n_heads, max_tokens,
+                                                           ctypes.byref(need)))
+            got = self._workspace_bytes[key] = need.value
         return got
 
 
@@ -230,7 +233,7 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
                    workspace=None, stream=None):
     """Attention of the batch's new tokens (already written) over the cache.  `mask`: int32 (tokens, words), bit i % 32
     of word i / 32 says whether the token sees new token i of its sequence; None: all up to and including itself.
-    `workspace`: a uint8 tensor of cache.attention_workspace(heads) bytes, used by one call at a time (allocated here
+    `workspace`: a uint8 tensor of cache.attention_workspace(heads, q.dtype, batch.max_tokens) bytes, used by one call at a time (allocated here
     when None)."""
     device, dtype = _device(q), act_dtype(q)
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
@@ -252,7 +255,7 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     if workspace is None:
         if stream is not None:
             _fail("a call on a stream of its own needs its own workspace")
-        workspace = torch.empty(cache.attention_workspace(heads), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens), dtype=torch.uint8, device=q.device)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
     rq, ro = _lib.Rows(q.data_ptr(), sq[0], sq[1]), _lib.Rows(out.data_ptr(), so[0], so[1])

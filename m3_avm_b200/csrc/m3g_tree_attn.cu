@@ -18,14 +18,6 @@
 // relative to a power of two dref >= every d seen by the warp; when it grows,
 // the sums are rescaled (rare).
 //
-// Work.  Sequences' lengths are only known on the device.  A unit is one
-// (sequence, KV head, row tile), cut into chunks of 128 positions; each CTA adds
-// up all chunks from the lengths and takes an equal, contiguous share, whatever
-// unit borders lie in it.  A unit inside one CTA is written out there; pieces of
-// a cut one go to the workspace, and k_tree_join adds them up in CTA order, so
-// the bits do not depend on timing.  One token of one long sequence is thus
-// spread over all SMs, and a ragged batch is balanced to one chunk.
-//
 // Inside a CTA each of 4 warps owns every fourth group of 32 positions and a
 // ring of stages filled by 16-byte cp.async; it keeps its own maximum, sum and
 // 16 x HD results in registers, so the warps meet only at the end of a piece.
@@ -34,8 +26,7 @@
 #include <cmath>
 #include <type_traits>
 
-#include "m3g_device.cuh"
-#include "m3g_serve.cuh"
+#include "m3g_tree.cuh"
 
 namespace m3g {
 namespace {
@@ -45,33 +36,6 @@ constexpr int kTreeThreads = 32 * kTreeWarps;
 constexpr int kGroup = 32;                      // positions per warp and step
 constexpr int kChunk = kGroup * kTreeWarps;     // positions per unit of work
 constexpr int kTile = 16;                       // rows per tile
-constexpr int kTreeCtasPerSm = 2;
-constexpr int kTreeMaxCtas = 2 * 160;           // CTAs that the workspace is sized for
-
-struct TreeArgs {
-  KvPlanes p;
-  m3g_kv_batch b;
-  m3g_rows q, out;
-  const uint32_t* mask;
-  float* parts;  // [2 * CTAs] of a tile's results, then its maxima and sums
-  int4* desc;    // [CTAs] the cut unit that starts in the CTA: sequence (-1: none), KV head, tile, its last CTA
-  long long cap;
-  int mask_words, n_heads, group;
-  int vec;       // q rows are 16-byte aligned
-  float scale;
-};
-
-template <int HD>
-struct Part {
-  static constexpr int kFloats = kTile * HD + 2 * kTile;
-};
-
-__device__ __forceinline__ float tex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -85,14 +49,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, __half2 off) {
   const uint32_t x = __byte_perm(w, 0x64646464u, SEL);  // 1024 + byte
   const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), off);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t x) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
 // Geometry of a warp's stage: K codes, V codes, K scales, V scales of 32 rows.
@@ -128,90 +84,24 @@ constexpr size_t tree_smem() {
   return ring > join ? ring : join;
 }
 
-__device__ __forceinline__ long long block_sum(long long v, long long* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int w = 0; w < kTreeWarps; ++w) v += red[w];
-  return v;
-}
-
-// Low n bits set, n clamped to 0 .. 32.
-__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-
-struct SeqWork {
-  SeqView v;
-  int chunks, tiles;  // chunks per unit, row tiles per KV head
-  __device__ __forceinline__ long long total(int kvh) const {
-    return static_cast<long long>(chunks) * tiles * kvh;
-  }
-};
-
-__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int s, bool* bad) {
-  SeqWork w;
-  w.v = seq_view(a.b, a.cap, s, bad);
-  w.chunks = w.v.n ? (w.v.ctx + w.v.n + kChunk - 1) / kChunk : 0;
-  w.tiles = static_cast<int>((static_cast<long long>(w.v.n) * a.group + kTile - 1) / kTile);
-  return w;
-}
-
 template <class T, int HD, bool Q8>
 __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(const __grid_constant__ TreeArgs a) {
   using St = Stage<HD, Q8>;
   constexpr bool SPLIT = std::is_same<T, float>::value;
   constexpr int NB = St::NB, NT = kGroup / 8, NO = HD / 8, KS = HD / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long red[kTreeWarps];
-  __shared__ long long found[2];  // the sequence of this CTA's first chunk, its chunks before it
+  __shared__ ShareScratch scratch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, t = lane & 3;
-  const int n_seqs = static_cast<int>(a.b.n_seqs), kvh = a.p.kvh;
-
-  // ---------------------------------------------------------------- this CTA's share
-  long long mine = 0;
+  const int kvh = a.p.kvh;
+  TreeShare share;
+  if (!tree_share<kChunk, kTile, kTreeThreads, 1>(a, scratch, share)) return;
   bool bad = false;
-  for (int s = tid; s < n_seqs; s += kTreeThreads) mine += seq_work(a, s, &bad).total(kvh);
-  if (bad && blockIdx.x == 0) atomicOr(a.p.status, kStatusBadBatch);
-  const long long W = block_sum(mine, red);
-  const long long G = gridDim.x < W ? gridDim.x : W;  // CTAs with work
-  if (tid == 0) a.desc[blockIdx.x].x = -1;
-  if (blockIdx.x >= G) return;
-  const long long first = blockIdx.x * W / G, last = (blockIdx.x + 1) * W / G;
-  {
-    long long before = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += kTreeThreads) {
-      const long long own = s0 + tid < n_seqs ? seq_work(a, s0 + tid, &bad).total(kvh) : 0;
-      long long up = own;  // inclusive scan
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xFFFFFFFFu, up, o);
-        if (lane >= o) up += x;
-      }
-      __syncthreads();
-      if (lane == 31) red[warp] = up;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) up += red[w];
-      const long long begin = before + up - own;
-      if (first >= begin && first < begin + own) {
-        found[0] = s0 + tid;
-        found[1] = begin;
-      }
-      long long all = 0;
-#pragma unroll
-      for (int w = 0; w < kTreeWarps; ++w) all += red[w];
-      before += all;
-      if (first < before) break;  // the same for all threads
-    }
-  }
-  __syncthreads();
-  int seq = static_cast<int>(found[0]);
-  SeqWork sw = seq_work(a, seq, &bad);
-  long long base_chunk = found[1];  // chunks of the sequences before this one
-  long long at = first;             // the next chunk
+  int seq = share.seq;
+  SeqWork<kChunk, kTile> sw(a, seq, &bad);
+  int base_chunk = share.before;  // chunks of the sequences before this one
+  int at = share.first;           // the next chunk
+  const int last = share.last;
 
   uint8_t* ring = smem + warp * St::kWarpBytes;
   const __half2 off = __half2half2(__ushort_as_half(Q8 ? 0x6480 : 0x6408));  // 1152, 1032
@@ -219,11 +109,11 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
   while (at < last) {
     while (at >= base_chunk + sw.total(kvh)) {
       base_chunk += sw.total(kvh);
-      sw = seq_work(a, ++seq, &bad);
+      sw = SeqWork<kChunk, kTile>(a, ++seq, &bad);
     }
-    const int in_seq = static_cast<int>((at - base_chunk) / sw.chunks);  // unit of the sequence
-    const int c0 = static_cast<int>((at - base_chunk) % sw.chunks);
-    const int c1 = static_cast<int>(min(static_cast<long long>(sw.chunks), c0 + (last - at)));
+    const int in_seq = (at - base_chunk) / sw.chunks;  // unit of the sequence
+    const int c0 = at - base_chunk - in_seq * sw.chunks;
+    const int c1 = min(sw.chunks, c0 + (last - at));
     const int head = in_seq / sw.tiles, tile = in_seq % sw.tiles;
     const int ctx = sw.v.ctx, len = sw.v.ctx + sw.v.n, rows = sw.v.n * a.group;
     const int32_t* table = a.b.page_table + static_cast<long long>(seq) * a.b.max_pages;
@@ -398,19 +288,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
       if (tail) {
         uint32_t vis[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int i0 = p0 - ctx;  // the first position as a new token's number
-          if (!a.mask) {
-            vis[i] = low_bits(token[i] + 1 - i0);
-          } else {
-            const uint32_t* mrow = a.mask + static_cast<long long>(sw.v.q0 + token[i]) * a.mask_words;
-            const int wd = i0 >> 5;  // floor: -1 and lower while context positions come first
-            const uint32_t lo = wd >= 0 && wd < a.mask_words ? mrow[wd] : 0u;
-            const uint32_t hi = wd + 1 >= 0 && wd + 1 < a.mask_words ? mrow[wd + 1] : 0u;
-            vis[i] = __funnelshift_r(lo, hi, i0 & 31) | low_bits(-i0);
-          }
-          vis[i] &= low_bits(len - p0);
-        }
+        for (int i = 0; i < 2; ++i) vis[i] = tree_sees(a, sw.v.q0, token[i], ctx, len, p0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -596,7 +474,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
             for (int e = 0; e < 4; ++e) y[d0 + 8 * d + e] = Act<T>::from(L == 0.f ? 0.f : O[d + e] * inv);
         }
       } else {
-        float* part = a.parts + static_cast<long long>(2 * blockIdx.x + (c0 == 0)) * Part<HD>::kFloats;
+        float* part = a.parts + static_cast<long long>(2 * blockIdx.x + (c0 == 0)) * Part<HD, kTile>::kFloats;
 #pragma unroll
         for (int d = 0; d < DPT; d += 4)
           *reinterpret_cast<float4*>(part + row * HD + d0 + 8 * d) = make_float4(O[d], O[d + 1], O[d + 2], O[d + 3]);
@@ -605,8 +483,8 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
           part[kTile * HD + kTile + row] = L;
         }
         if (tid == 0 && c0 == 0) {
-          const long long end = base_chunk + static_cast<long long>(in_seq + 1) * sw.chunks;  // the unit's end
-          a.desc[blockIdx.x] = make_int4(seq, head, tile, static_cast<int>((end * G - 1) / W));
+          const int end = base_chunk + (in_seq + 1) * sw.chunks;  // the unit's end
+          a.desc[blockIdx.x] = make_int4(seq, head, tile, tree_last_cta(share, end));
         }
       }
     }
@@ -614,48 +492,6 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
     at += c1 - c0;
   }
   grid_dep_launch();
-}
-
-// The pieces of the units that were cut, in CTA order: one CTA per main CTA,
-// one warp per row.
-template <class T, int HD>
-__global__ void __launch_bounds__(32 * kTile) k_tree_join(const __grid_constant__ TreeArgs a) {
-  constexpr int DPL = HD / 32;
-  grid_dep_wait();
-  const int4 u = a.desc[blockIdx.x];
-  if (u.x < 0) return;
-  const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  bool bad = false;
-  const SeqView s = seq_view(a.b, a.cap, u.x, &bad);
-  const int grow_row = u.z * kTile + row;
-  if (grow_row >= s.n * a.group) return;
-  const int n = u.w - static_cast<int>(blockIdx.x) + 1;  // pieces
-  auto part = [&](int i) {  // this CTA's piece starts the unit, the others continue it
-    return a.parts + static_cast<long long>(i ? 2 * (blockIdx.x + i) : 2 * blockIdx.x + 1) * Part<HD>::kFloats;
-  };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[kTile * HD + row]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f, O[DPL];
-#pragma unroll
-  for (int d = 0; d < DPL; ++d) O[d] = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) {
-    const float* p = part(i);
-    const float f = tex2(p[kTile * HD + row] - ref);
-    L += f * p[kTile * HD + kTile + row];
-    float v[DPL];
-    load_act<float, DPL, true>(p + row * HD + lane * DPL, v);
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) O[d] += f * v[d];
-  }
-  T* y = static_cast<T*>(a.out.p) + (s.q0 + grow_row / a.group) * a.out.token_stride +
-         (u.y * a.group + grow_row % a.group) * a.out.head_stride;
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-  for (int d = 0; d < DPL; ++d) y[lane * DPL + d] = Act<T>::from(L == 0.f ? 0.f : O[d] * inv);
 }
 
 template <class T, int HD, bool Q8>
@@ -667,12 +503,23 @@ cudaError_t launch_tree(const TreeArgs& a, int sms, cudaStream_t st) {
   const int grid = std::min(kTreeMaxCtas, kTreeCtasPerSm * sms);
   e = serve_launch(k_tree_attn<T, HD, Q8>, dim3(grid), dim3(kTreeThreads), smem, st, false, a);
   if (e != cudaSuccess || a.cap <= kChunk) return e;  // one chunk per unit: none is cut
-  return serve_launch(k_tree_join<T, HD>, dim3(grid), dim3(32 * kTile), 0, st, true, a);
+  return launch_join<T, HD, kTile>(a, grid, st);
 }
 template <class T>
 cudaError_t launch_tree_t(const TreeArgs& a, bool q8, int sms, cudaStream_t st) {
   if (a.p.hd == 64) return q8 ? launch_tree<T, 64, true>(a, sms, st) : launch_tree<T, 64, false>(a, sms, st);
   return q8 ? launch_tree<T, 128, true>(a, sms, st) : launch_tree<T, 128, false>(a, sms, st);
+}
+
+// Which form: the one of 128-row tiles (m3g_tree_umma.cu) for 16-bit types where
+// a KV head has more than 48 rows and there are 8 chunks for each of its CTAs.
+// Measured (32 query over 8 KV heads of 128, Q8_0, bf16): 8 sequences of up to 8000
+// positions, 48 rows 78 against 76 us here, 64 rows 79 against 93, 256 rows 112
+// against 280; one sequence of 2000 positions (1 chunk for each CTA) 29 against
+// some 17 us at 48 rows, 41 against 33 at 256.
+constexpr uint64_t kUmmaRows = 49, kUmmaChunks = 8 * 296;
+bool can_use_umma(const m3g_kv_layout* l, uint32_t dtype, uint32_t n_heads, uint32_t max_tokens) {
+  return dtype != M3G_DTYPE_F32 && static_cast<uint64_t>(max_tokens) * (n_heads / l->n_kv_heads) >= kUmmaRows;
 }
 
 int check_heads(const m3g_kv_layout* l, uint32_t n_heads) {
@@ -686,13 +533,15 @@ int check_heads(const m3g_kv_layout* l, uint32_t n_heads) {
 
 extern "C" {
 
-M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* l, uint32_t n_heads, uint64_t* out) {
+M3G_API int m3g_tree_attn_workspace(const m3g_kv_layout* l, uint32_t dtype, uint32_t n_heads, uint32_t max_tokens,
+                                    uint64_t* out) {
   if (!out) return m3g::host_fail(M3G_EINVAL, "null argument");
   *out = 0;
   if (int rc = m3g::kv_check(l)) return rc;
   if (int rc = m3g::check_heads(l, n_heads)) return rc;
-  const uint64_t part = sizeof(float) * (l->head_dim == 64 ? m3g::Part<64>::kFloats : m3g::Part<128>::kFloats);
-  *out = m3g::kTreeMaxCtas * (sizeof(int4) + 2 * part);
+  if (!m3g::act_size(dtype)) return m3g::host_fail(M3G_EINVAL, "attention of dtype %u (F32, F16 and BF16 are supported)", dtype);
+  const uint64_t tile = m3g::can_use_umma(l, dtype, n_heads, max_tokens) ? m3g::kUmmaTile : m3g::kTile;
+  *out = m3g::kTreeMaxCtas * (sizeof(int4) + 2 * sizeof(float) * tile * (l->head_dim + 2));
   return M3G_OK;
 }
 
@@ -720,7 +569,7 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   if (mask && static_cast<uint64_t>(mask_words) * 32 < b->max_tokens)
     return host_fail(M3G_EINVAL, "%u mask words for %u tokens", mask_words, b->max_tokens);
   uint64_t need = 0;
-  if (int rc = m3g_tree_attn_workspace(l, n_heads, &need)) return rc;
+  if (int rc = m3g_tree_attn_workspace(l, dtype, n_heads, b->max_tokens, &need)) return rc;
   if (!b->n_tokens || !b->n_seqs) return M3G_OK;
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
     return host_fail(M3G_EINVAL, "workspace of %llu bytes (16-byte aligned, %llu needed)",
@@ -732,6 +581,7 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   a.desc = static_cast<int4*>(workspace);
   a.parts = reinterpret_cast<float*>(a.desc + kTreeMaxCtas);
   a.vec = rows_aligned(q->p, q->token_stride, q->head_stride, size);
+  a.vec_out = rows_aligned(out->p, out->token_stride, out->head_stride, size);
   a.b = *b;
   a.q = *q;
   a.out = *out;
@@ -740,10 +590,19 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   a.cap = seq_cap(*b, l->page_size);
   a.n_heads = static_cast<int>(n_heads);
   a.group = static_cast<int>(n_heads / l->n_kv_heads);
+  // chunks of 64 positions at worst, in tiles of 16 rows
+  const uint64_t units = static_cast<uint64_t>(b->n_seqs) * l->n_kv_heads *
+                         ((static_cast<uint64_t>(b->max_tokens) * a.group + kTile - 1) / kTile);
+  if (static_cast<uint64_t>(b->max_tokens) * a.group >= (1ull << 31) || units >= (1ull << 31) || units * (static_cast<uint64_t>(a.cap) / 64 + 1) >= (1ull << 31))
+    return host_fail(M3G_EINVAL, "batch too large (sequences x heads x tokens x length)");
+  const uint64_t tiles = (static_cast<uint64_t>(b->max_tokens) * a.group + kUmmaTile - 1) / kUmmaTile;
+  const bool umma = can_use_umma(l, dtype, n_heads, b->max_tokens) &&
+                    b->n_seqs * l->n_kv_heads * tiles * ((static_cast<uint64_t>(a.cap) + 63) / 64) >= kUmmaChunks;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(a.p.hd));
   const cudaStream_t st = serve_stream(stream);
   const bool q8 = l->dtype == M3G_DTYPE_Q8_0;
-  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_tree_t<float>(a, q8, sms, st)
+  const cudaError_t e = umma ? launch_tree_umma(a, dtype, q8, sms, st)
+                        : dtype == M3G_DTYPE_F32 ? launch_tree_t<float>(a, q8, sms, st)
                         : dtype == M3G_DTYPE_F16 ? launch_tree_t<__half>(a, q8, sms, st)
                                                  : launch_tree_t<__nv_bfloat16>(a, q8, sms, st);
   if (e != cudaSuccess) return host_fail(M3G_ECUDA, "k_tree_attn: %s", cudaGetErrorString(e));

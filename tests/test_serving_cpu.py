@@ -100,7 +100,7 @@ def test_cache_layout_refusals(lib, bad):
     assert lib.m3g_kv_bytes(ctypes.byref(layout(**bad)), ctypes.byref(out)) == EINVAL
     assert out.value == 0
     ws = ctypes.c_uint64(7)
-    assert lib.m3g_tree_attn_workspace(ctypes.byref(layout(**bad)), 8, ctypes.byref(ws)) == EINVAL
+    assert lib.m3g_tree_attn_workspace(ctypes.byref(layout(**bad)), 0, 8, 1, ctypes.byref(ws)) == EINVAL
 
 
 def test_cache_too_large(lib):

@@ -273,11 +273,22 @@ def test_cache_bad_pages_and_batches():
 
 
 # ---------------------------------------------------------------- attention
+def roomy(batch, page):
+    """The same batch with limits of 2^18 positions: large trees then take the form for large calls."""
+    from m3_avm_b200.attention import KvBatch
+
+    table = torch.full((batch.page_table.shape[0], 2 ** 18 // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :batch.page_table.shape[1]] = batch.page_table
+    return KvBatch(batch.q_start, batch.ctx_len, table, batch.n_tokens, batch.max_tokens, 2 ** 18)
+
+
 def attention_case(q8, dtype, heads, kvh, hd, page, ctx, new, tree, seed=0, empty=(), qscale=1.5, strided=False,
-                   scale=None, cache=None):
+                   scale=None, large=False):
     from m3_avm_b200.attention import KvCache, tree_attention
 
     batch, pages, _, _ = R.make_batch(ctx, new, page, seed=seed)
+    if large:
+        batch = roomy(batch, page)
     cache = KvCache(8 if q8 else 2, 2, kvh, hd, page, pages)
     cache.pool.fill_(0xFF)  # rows behind the sequences: scales that are NaN
     full = R.whole(batch, ctx, new)
@@ -336,10 +347,48 @@ def test_attention_long_and_many(dtype):
 
 
 @pytest.mark.parametrize("q8", [True, False])
-def test_attention_large_trees(q8):
-    for dtype, new in ((BF16, [64, 50, 17]), (F16, [64]), (F32, [40, 40]), (BF16, [257])):
-        got, want, bound, _ = attention_case(q8, dtype, 16, 2, 128, 64, [777, 0, 64][:len(new)], new, True, seed=4)
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_large_trees(q8, large, hd):
+    for dtype, new in ((BF16, [64, 50, 17]), (F16, [64]), (F32, [40, 40]), (BF16, [257]), (F16, [7, 33])):
+        got, want, bound, _ = attention_case(q8, dtype, 16, 2, hd, 64, [777, 0, 64][:len(new)], new, True, seed=4,
+                                             large=large)
         assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kvh,page,ctx,new,tree", [
+    (64, 8, 16, [0], [9], False), (64, 1, 16, [63], [1], False), (64, 1, 64, [64, 0, 1, 127], [1, 2, 1, 65], True),
+    (10, 2, 32, [3000, 100, 5], [30, 1, 12], True), (32, 1, 128, [20000], [3], True),
+])
+def test_attention_large_form(dtype, heads, kvh, page, ctx, new, tree):
+    for q8 in (True, False):
+        got, want, bound, (q, cache, batch, mask) = attention_case(q8, dtype, heads, kvh, 128, page, ctx, new, tree,
+                                                                   seed=kvh, large=True)
+        assert_within(got, want, bound)
+        from m3_avm_b200.attention import tree_attention
+
+        for _ in range(3):
+            assert torch.equal(tree_attention(q, cache, 1, batch, mask=mask), got)
+
+
+def test_attention_large_form_growing_scores():
+    """Maxima that grow by 2^20 from one chunk to the next: the results so far are rescaled each time."""
+    from m3_avm_b200.attention import KvCache, tree_attention
+
+    for dtype in (F16, BF16):
+        batch, pages, _, _ = R.make_batch([700], [20], 16)
+        cache = KvCache(8, 1, 1, 64, 16, pages)
+        full = R.whole(batch, [700], [20])
+        k, v = randn(1, 720, 1, 64, scale=0.1), randn(2, 720, 1, 64)
+        q = randn(3, 20, 4, 64, dtype=dtype)
+        k += (torch.arange(720, device="cuda") // 64 * 0.25).view(-1, 1, 1) * torch.sign(q[3, 1].float())
+        cache.write(0, k, v, full)
+        got = tree_attention(q, cache, 0, roomy(batch, 16), scale=1.0)
+        bits = [np.tril(np.ones((20, 20), bool))]
+        want, vmax, smag = R.attention(q, [R.quantised(k, True).double()], [R.quantised(v, True).double()], [700], [20],
+                                       bits, 1.0)
+        assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
 
 
 def test_attention_rows_that_see_nothing():
@@ -352,8 +401,10 @@ def test_attention_what_a_row_does_not_see_does_not_reach_it():
     """A drafted token whose K or V is NaN leaves the rows that do not see it as they were."""
     from m3_avm_b200.attention import KvCache, tree_attention
 
-    for hd, dtype, heads in ((64, F32, 4), (128, BF16, 4), (128, BF16, 64)):
+    for hd, dtype, heads, large in ((64, F32, 4, False), (128, BF16, 4, False), (128, BF16, 64, False),
+                                    (128, BF16, 64, True), (64, F16, 64, True)):
         batch, pages, _, _ = R.make_batch([20], [6], 16)
+        batch = roomy(batch, 16) if large else batch
         cache = KvCache(8, 1, 2, hd, 16, pages)
         full = R.whole(batch, [20], [6])
         k, v = randn(1, 26, 2, hd), randn(2, 26, 2, hd)
@@ -384,12 +435,12 @@ def test_attention_what_a_row_does_not_see_does_not_reach_it():
 def test_attention_strides_in_place_and_scale():
     from m3_avm_b200.attention import tree_attention
 
-    for dtype in (F32, F16):
-        got, want, bound, (q, cache, batch, mask) = attention_case(True, dtype, 8, 2, 128, 16, [50], [5], True, seed=6,
-                                                                   strided=True, scale=0.2)
+    for dtype, heads, large in ((F32, 8, False), (F16, 8, False), (F16, 32, True), (BF16, 32, True)):
+        got, want, bound, (q, cache, batch, mask) = attention_case(True, dtype, heads, 2, 128, 16, [50], [5], True,
+                                                                   seed=6, strided=True, scale=0.2, large=large)
         assert_within(got, want, bound)
-        buf = torch.zeros(5 * 8 * 131 + 1, dtype=dtype, device="cuda")
-        odd = buf.as_strided((5, 8, 128), (8 * 131, 131, 1), 1)
+        buf = torch.zeros(5 * heads * 131 + 1, dtype=dtype, device="cuda")
+        odd = buf.as_strided((5, heads, 128), (heads * 131, 131, 1), 1)
         odd.copy_(q)
         assert torch.equal(tree_attention(odd, cache, 1, batch, mask=mask, scale=0.2), got)
         assert tree_attention(odd, cache, 1, batch, mask=mask, scale=0.2, out=odd) is odd
@@ -433,31 +484,34 @@ def test_attention_bad_page_reads_as_zeros():
 def test_attention_of_large_and_tiny_values():
     from m3_avm_b200.attention import KvCache, tree_attention
 
-    for dtype in (F32, BF16):
+    for dtype, large in ((F32, False), (BF16, False), (BF16, True)):
         for scale_v in (3e5, 1e-6):
             batch, pages, _, _ = R.make_batch([100], [3], 16)
+            heads = 64 if large else 4
             cache = KvCache(8, 1, 1, 64, 16, pages)
             full = R.whole(batch, [100], [3])
             k, v = randn(1, 103, 1, 64, scale=20.0), randn(2, 103, 1, 64, scale=scale_v)
             v[50:] *= 1e-3 if scale_v > 1 else 1.0
             cache.write(0, k, v, full)
-            q = randn(3, 3, 4, 64, scale=2.0, dtype=dtype)
-            got = tree_attention(q, cache, 0, batch)
+            q = randn(3, 3, heads, 64, scale=2.0, dtype=dtype)
+            got = tree_attention(q, cache, 0, roomy(batch, 16) if large else batch)
             bits = [np.tril(np.ones((3, 3), bool))]
             want, vmax, smag = R.attention(q, [R.quantised(k, True).double()], [R.quantised(v, True).double()], [100],
                                            [3], bits, 0.125)
             assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
 
 
-def test_attention_repeats_to_the_bit_and_replays_from_a_graph():
+@pytest.mark.parametrize("heads,large", [(8, False), (64, True)])
+def test_attention_repeats_to_the_bit_and_replays_from_a_graph(heads, large):
     from m3_avm_b200.attention import tree_attention
 
-    _, _, _, (q, cache, batch, mask) = attention_case(True, BF16, 8, 2, 128, 16, [3000, 20], [5, 6], True, seed=3)
+    _, _, _, (q, cache, batch, mask) = attention_case(True, BF16, heads, 2, 128, 16, [3000, 20], [5, 6], True, seed=3,
+                                                      large=large)
     first = tree_attention(q, cache, 1, batch, mask=mask)
     for _ in range(3):
         assert torch.equal(tree_attention(q, cache, 1, batch, mask=mask), first)
     out = torch.zeros_like(q)
-    ws = torch.empty(cache.attention_workspace(8), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(cache.attention_workspace(heads, BF16, 6), dtype=torch.uint8, device="cuda")
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -481,7 +535,7 @@ def test_attention_two_streams_at_once():
     from m3_avm_b200.attention import tree_attention
 
     a = attention_case(True, F32, 8, 2, 64, 16, [5000], [3], True, seed=3)
-    b = attention_case(False, F16, 12, 4, 128, 16, [7000], [9], True, seed=5)
+    b = attention_case(False, F16, 64, 4, 128, 16, [7000], [9], True, seed=5, large=True)
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
     outs = []
