@@ -43,6 +43,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same into a new sum.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Bytes SEL picks of w (two of them), less `off`, as exact f16 values.
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t codes2(uint32_t w, __half2 off) {
@@ -51,15 +59,27 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, __half2 off) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// CTAs per SM: what their registers leave room for without spills in the loop.
+// With 64 values a row three (12 warps of 168 registers; 8 contexts of 8000
+// positions and 16 tokens: 27.0 us, with two 28.0; F32, 256 tokens: 195 us, with two
+// 214).  With 128 values two: three need 26 KB of stages instead of 48 and gain
+// nothing, since the ALU pipe is what is short and not warps to issue from (48
+// ragged contexts of up to 16000 positions: 246 us, with three 249).
+template <int HD>
+struct Ctas {
+  static constexpr int kPerSm = HD == 128 ? 2 : 3;
+};
+
 // Geometry of a warp's stage: K codes, V codes, K scales, V scales of 32 rows.
-template <int HD, bool Q8>
+template <int HD, bool Q8, int CTAS>
 struct Stage {
   static constexpr int CB = Q8 ? HD : HD / 2, SB = HD / 16, NB = HD / 32;
   static constexpr int CPR = CB / 16;   // 16-byte pieces per row
   static constexpr int RPL = 128 / CB;  // rows per 128-byte line
   static constexpr int kCodes = kGroup * CB, kScales = kGroup * SB;
   static constexpr int kBytes = 2 * (kCodes + kScales);
-  static constexpr int NS = 26112 / kBytes < 8 ? 26112 / kBytes : 8;  // stages: 3 for the largest rows
+  static constexpr int kRoom = CTAS == 2 ? 26112 : 18432;  // shared memory of a warp
+  static constexpr int NS = kRoom / kBytes < 8 ? kRoom / kBytes : 8;
   static constexpr int kWarpBytes = NS * kBytes;
   // Byte offset of 16-byte piece `col` of `row`.  K fragments read one block of
   // 8 rows at once, V fragments one block of rows 2t (t = 0..3).
@@ -77,16 +97,16 @@ struct Stage {
   }
 };
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, int CTAS>
 constexpr size_t tree_smem() {
-  const size_t ring = static_cast<size_t>(kTreeWarps) * Stage<HD, Q8>::kWarpBytes;
+  const size_t ring = static_cast<size_t>(kTreeWarps) * Stage<HD, Q8, CTAS>::kWarpBytes;
   const size_t join = sizeof(float) * kTreeWarps * kTile * (HD + 4 + 2);
   return ring > join ? ring : join;
 }
 
 template <class T, int HD, bool Q8>
-__global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(const __grid_constant__ TreeArgs a) {
-  using St = Stage<HD, Q8>;
+__global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(const __grid_constant__ TreeArgs a) {
+  using St = Stage<HD, Q8, Ctas<HD>::kPerSm>;
   constexpr bool SPLIT = std::is_same<T, float>::value;
   constexpr int NB = St::NB, NT = kGroup / 8, NO = HD / 8, KS = HD / 16;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -198,7 +218,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
       most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
       // times a power of two that puts the largest into [2^10, 2^11)
-      const int e = max(11, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
+      const int e = max(60, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
       const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23);
       row_scale[i] = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 10) << 23);
 #pragma unroll
@@ -235,7 +255,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
       const uint8_t* kscales = st + 2 * St::kCodes;
       const uint8_t* vscales = kscales + St::kScales;
 
-      float s[NT][4];
+      uint64_t s2[NT][2];  // raw scores of positions 8nt + 2t, + 1; of rows r, r + 8
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int row = 8 * nt + r;
@@ -247,12 +267,12 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
           const uint2 x = *reinterpret_cast<const uint2*>(kscales + (8 * nt + 2 * t) * St::SB);
           dk[0] = x.x; dk[1] = x.y;
         }
-        float d0[NB], d1[NB];
+        uint64_t dd[NB];  // of the two positions
 #pragma unroll
         for (int h = 0; h < NB / 2; ++h) {
           const float2 x = unpack_f16(dk[h]), y = unpack_f16(dk[NB / 2 + h]);
-          d0[2 * h] = x.x; d0[2 * h + 1] = x.y;
-          d1[2 * h] = y.x; d1[2 * h + 1] = y.y;
+          dd[2 * h] = pair(x.x, y.x);
+          dd[2 * h + 1] = pair(x.y, y.y);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -266,21 +286,20 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
             w[0] = x & 0x0F0F0F0Fu;
             w[1] = (x >> 4) & 0x0F0F0F0Fu;
           }
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          float acc[4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t b0 = codes2<0x4140>(w[h], off), b1 = codes2<0x4342>(w[h], off);
-            mma_f16(acc, qh[2 * b + h], b0, b1);
+            if (h) mma_f16(acc, qh[2 * b + h], b0, b1);
+            else mma_f16_first(acc, qh[2 * b], b0, b1);
             if (SPLIT) mma_f16(acc, ql[SPLIT ? 2 * b + h : 0], b0, b1);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float d = e & 1 ? d1[b] : d0[b];
-            s[nt][e] = b ? fmaf(d, acc[e], s[nt][e]) : d * acc[e];
+          for (int i = 0; i < 2; ++i) {
+            const uint64_t x = pair(acc[2 * i], acc[2 * i + 1]);
+            s2[nt][i] = b ? fma2(dd[b], x, s2[nt][i]) : mul2(dd[b], x);
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] *= row_scale[e >> 1];
       }
 
       // ------------------------------------------------------------ mask
@@ -292,8 +311,10 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(vis[e >> 1] >> (8 * nt + 2 * t + (e & 1)) & 1u)) s[nt][e] = -INFINITY;
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t v = vis[i] >> (8 * nt + 2 * t);
+            s2[nt][i] = pair(v & 1u ? low(s2[nt][i]) : -INFINITY, v & 2u ? high(s2[nt][i]) : -INFINITY);
+          }
       }
 
       // ------------------------------------------------------------ softmax
@@ -301,14 +322,14 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[nt][e]);
+        for (int i = 0; i < 2; ++i) top[i] = max3(top[i], low(s2[nt][i]), high(s2[nt][i]));
       float ref[2], grow[2];
       bool grew = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
         top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
-        const float mn = fmaxf(m[i], top[i]);
+        const float mn = fmaxf(m[i], top[i] * row_scale[i]);
         ref[i] = mn == -INFINITY ? 0.f : mn;
         grow[i] = tex2(m[i] - ref[i]);
         grew = grew || mn > m[i];
@@ -344,18 +365,25 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][e] *= grow[e >> 1] * shrink;
       }
+      // Weights times 2^14 / dref, a power of two, so that times V's scales they are
+      // at most 2^14.
+      const int lift = 14 + 127 - static_cast<int>(__float_as_uint(dref) >> 23);
+      const float unlift = dref * 0x1p-14f;
+      uint64_t sum2[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) l[i] *= grow[i];
+      for (int i = 0; i < 2; ++i) {
+        const float c0 = static_cast<float>(lift) - ref[i];
+        const uint64_t rs2 = pair(row_scale[i], row_scale[i]), c2 = pair(c0, c0);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nt][e] = tex2(s[nt][e] - ref[e >> 1]);
-          l[e >> 1] += s[nt][e];
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint64_t x = fma2(s2[nt][i], rs2, c2);
+          s2[nt][i] = pair(tex2(low(x)), tex2(high(x)));
+          sum2[i] = add2(sum2[i], s2[nt][i]);
         }
+        l[i] = l[i] * grow[i] + (low(sum2[i]) + high(sum2[i])) * unlift;
+      }
 
       // ------------------------------------------------------------ values
-      const float dinv = 0x1p14f / dref;  // p * d * dinv <= 2^14
 #pragma unroll
       for (int kk = 0; kk < kGroup / 16; ++kk) {
         uint32_t vw[NB][4];  // codes of positions 16kk + {2t, 2t + 1, 2t + 8, 2t + 9}, four dims of each block
@@ -364,12 +392,8 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int row = 16 * kk + 2 * t + (k & 1) + 8 * (k >> 1);
-            if (Q8) {
-              vw[b][k] = *reinterpret_cast<const uint32_t*>(vcodes + St::v_at(row, 2 * b + (r >> 2)) + (r & 3) * 4);
-            } else {
-              const uint32_t x = *reinterpret_cast<const uint32_t*>(vcodes + St::v_at(row, b) + (r & 3) * 4);
-              vw[b][k] = (x >> (r & 4)) & 0x0F0F0F0Fu;
-            }
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(vcodes + St::v_at(row, Q8 ? 2 * b + (r >> 2) : b) + (r & 3) * 4);
+            vw[b][k] = Q8 ? x : (x >> (r & 4)) & 0x0F0F0F0Fu;
           }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -378,13 +402,14 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
           for (int h = 0; h < 2; ++h) {  // positions 16kk + 8h + 2t, + 1
             const int nt = 2 * kk + h;
             const float2 x = unpack_f16(dv[nt][b / 2]), y = unpack_f16(dv[nt][NB / 2 + b / 2]);
-            const float e0 = (b & 1 ? x.y : x.x) * dinv, e1 = (b & 1 ? y.y : y.x) * dinv;
+            const uint64_t e = b & 1 ? pair(x.y, y.y) : pair(x.x, y.x);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float w0 = s[nt][2 * i] * e0, w1 = s[nt][2 * i + 1] * e1;
+              const uint64_t w = mul2(s2[nt][i], e);
+              float w0 = low(w), w1 = high(w);
               if (tail) {  // a position that the row does not see adds nothing, NaN or not
-                w0 = s[nt][2 * i] == 0.f ? 0.f : w0;
-                w1 = s[nt][2 * i + 1] == 0.f ? 0.f : w1;
+                w0 = low(s2[nt][i]) == 0.f ? 0.f : w0;
+                w1 = high(s2[nt][i]) == 0.f ? 0.f : w1;
               }
               const uint32_t hi = pack_f16(w0, w1);
               ph[2 * h + i] = hi;
@@ -496,11 +521,11 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm) k_tree_attn(cons
 
 template <class T, int HD, bool Q8>
 cudaError_t launch_tree(const TreeArgs& a, int sms, cudaStream_t st) {
-  constexpr size_t smem = tree_smem<HD, Q8>();
+  constexpr size_t smem = tree_smem<HD, Q8, Ctas<HD>::kPerSm>();
   cudaError_t e = cudaFuncSetAttribute(k_tree_attn<T, HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  const int grid = std::min(kTreeMaxCtas, kTreeCtasPerSm * sms);
+  const int grid = std::min(kTreeMaxCtas, Ctas<HD>::kPerSm * sms);
   e = serve_launch(k_tree_attn<T, HD, Q8>, dim3(grid), dim3(kTreeThreads), smem, st, false, a);
   if (e != cudaSuccess || a.cap <= kChunk) return e;  // one chunk per unit: none is cut
   return launch_join<T, HD, kTile>(a, grid, st);

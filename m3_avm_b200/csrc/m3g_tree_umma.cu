@@ -86,28 +86,6 @@ __device__ __forceinline__ void tc_ld_wait(uint32_t (&x)[16]) {
                : "memory");
 }
 
-// Two f32 operations in one instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  return static_cast<uint64_t>(__float_as_uint(lo)) | static_cast<uint64_t>(__float_as_uint(hi)) << 32;
-}
-__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float(static_cast<uint32_t>(x)); }
-__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float(static_cast<uint32_t>(x >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 template <int HD, bool Q8, bool SPLIT>
 struct UGeo {
   static constexpr int CB = Q8 ? HD : HD / 2, SB = HD / 16, NB = HD / 32, CPR = CB / 16;
@@ -365,7 +343,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
             }
           }
         }
-        const int e = max(5, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
+        const int e = max(60, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
         const float up = __uint_as_float(static_cast<uint32_t>(258 - e) << 23);
         cs = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 4) << 23);
 #pragma unroll 1
@@ -706,7 +684,7 @@ cudaError_t launch_umma(const TreeArgs& a, int sms, cudaStream_t st) {
   const auto kern = k_tree_umma<T, HD, Q8, SPLIT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const int grid = kTreeCtasPerSm * sms < kTreeMaxCtas ? kTreeCtasPerSm * sms : kTreeMaxCtas;
+  const int grid = 2 * sms < kTreeMaxCtas ? 2 * sms : kTreeMaxCtas;
   e = serve_launch(kern, dim3(grid), dim3(kUThreads), smem, st, false, a);
   if (e != cudaSuccess || a.cap <= kUChunk) return e;  // one chunk per unit: none is cut
   return launch_join<T, HD, kUmmaTile>(a, grid, st);
