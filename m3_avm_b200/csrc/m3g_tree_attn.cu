@@ -536,15 +536,19 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool q8, int sms, cudaStream_t st) 
   return q8 ? launch_tree<T, 128, true>(a, sms, st) : launch_tree<T, 128, false>(a, sms, st);
 }
 
-// Which form: the one of 128-row tiles (m3g_tree_umma.cu) for 16-bit types where
-// a KV head has more than 48 rows and there are 8 chunks for each of its CTAs.
-// Measured (32 query over 8 KV heads of 128, Q8_0, bf16): 8 sequences of up to 8000
-// positions, 48 rows 78 against 76 us here, 64 rows 79 against 93, 256 rows 112
-// against 280; one sequence of 2000 positions (1 chunk for each CTA) 29 against
-// some 17 us at 48 rows, 41 against 33 at 256.
-constexpr uint64_t kUmmaRows = 49, kUmmaChunks = 8 * 296;
+// Which form: the one of 128-row tiles (m3g_tree_umma.cu) for 16-bit types where a
+// KV head has more than 64 rows (48 for BF16 of 128 values, which needs no second
+// part of K) and there are 8 chunks for each of its CTAs.  Measured, that form
+// against this one (32 query over 8 KV heads, Q8_0, 8 sequences of up to 8000
+// positions): BF16 of 128 values, 48 rows 75 against 71 us, 56 rows 76 against 78,
+// 256 rows 112 against 260; F16 of 128, 64 rows 93 against 88, 128 rows 100 against
+// 143; 64 values, 64 rows 57 against 55, 128 rows 61 against 90.  With fewer chunks
+// (2 sequences of 8000, 128 rows, 2000 chunks) 73 against 56 us; one sequence of
+// 2000 positions, 256 rows, 39 against 29.
+constexpr uint64_t kUmmaChunks = 8 * 296;
 bool can_use_umma(const m3g_kv_layout* l, uint32_t dtype, uint32_t n_heads, uint32_t max_tokens) {
-  return dtype != M3G_DTYPE_F32 && static_cast<uint64_t>(max_tokens) * (n_heads / l->n_kv_heads) >= kUmmaRows;
+  const uint64_t least = dtype == M3G_DTYPE_BF16 && l->head_dim == 128 ? 49 : 65;
+  return dtype != M3G_DTYPE_F32 && static_cast<uint64_t>(max_tokens) * (n_heads / l->n_kv_heads) >= least;
 }
 
 int check_heads(const m3g_kv_layout* l, uint32_t n_heads) {

@@ -661,6 +661,37 @@ def test_logprobs_rows_without_a_distribution():
     assert int(got.top_ids[3, 0]) == 2999
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab", [(1, 60001), (700, 300)])
+def test_logprobs_rows_of_extreme_logits(dtype, rows, vocab):
+    """Rows with nothing above the type's lowest value, and rows up to its largest: all but the largest logits have
+    probability 0 there, so a log probability is -ln(how many), of which log2, the product with ln 2 and its constant
+    are rounded.  A largest logit below 1e38 (F16: above -32768) has the term 2^d, d the rounding of its product with
+    log2(e): ex2 is off by 2^-22 and their sum by (n / 512 + 32) 2^-24 of itself."""
+    from m3_avm_b200.logprobs import token_logprobs
+
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    tol = 3 * 2.0 ** -22 * math.log(vocab) + 2.0 ** -22 + (vocab / 512 + 32) * 2.0 ** -24
+    some = torch.arange(vocab) % 3 == 1
+    for fill, value in ((low, low), (-math.inf, low), (low, 0.75 * low), (0.75 * low, 0.5 * low), (low, high), (0, high),
+                        (-math.inf, high), (0.75 * high, high)):
+        x = torch.where(some, torch.tensor(value, dtype=dtype), torch.tensor(fill, dtype=dtype)).expand(rows, vocab)
+        x = x.contiguous()
+        tokens = torch.tensor([[1, 4, 0]], dtype=torch.int32).expand(rows, 3).contiguous()
+        got = token_logprobs(x.cuda(), tokens.cuda(), n_top=5, entropy=True)
+        given, entropy, ids, tops = logprob_reference(x, tokens, 5)
+        assert torch.equal(got.top_ids.cpu().long(), ids)
+        for a, b in ((got.logprob, given), (got.top_logprobs, tops), (got.entropy, entropy)):
+            a = a.double().cpu()
+            far = b < -200.0  # differences of logits: one rounding, or past the type
+            assert bool(((a - b).abs()[~far] <= tol).all())
+            assert bool(((a[far] <= b[far] * (1 - 2.0 ** -20)) & (a[far] < -200.0)).all())
+    y = torch.full((2, vocab), low, dtype=dtype)
+    y[0, 7], y[1, vocab - 1] = float("nan"), math.inf
+    got = token_logprobs(y.cuda(), torch.zeros(2, 1, dtype=torch.int32).cuda(), n_top=3, entropy=True)
+    assert torch.isnan(got.logprob).all() and torch.isnan(got.entropy).all() and torch.isnan(got.top_logprobs).all()
+
+
 def test_logprobs_strides_and_unaligned_rows():
     from m3_avm_b200.logprobs import token_logprobs
 
