@@ -286,6 +286,15 @@ M3G_API int m3g_decoder_forward(m3g_decoder* dec, uint32_t token, float* logits)
  * last step's logits to the host when `logits` is not NULL.  Afterwards the
  * greedy pick of those logits is pending as the next token. */
 M3G_API int m3g_decoder_prefill(m3g_decoder* dec, const uint32_t* tokens, uint64_t n, float* logits);
+/* Prefill that also says how probable the tokens were: entry i is about the
+ * distribution that follows tokens[i].  logprob [n]: of tokens[i + 1], the last
+ * one of the pending greedy pick; entropy [n]; the n_top (<= 32) most probable
+ * ids with their log probabilities, [n][n_top] each.  Host pointers, NULL for
+ * what is not wanted (top_id and top_logprob with n_top 0).  Numbers as
+ * m3g_token_logprobs_dev gives them; the KV cache, the logits and the pick are
+ * those of m3g_decoder_prefill. */
+M3G_API int m3g_decoder_score(m3g_decoder* dec, const uint32_t* tokens, uint64_t n, float* logprob, float* entropy,
+                              uint32_t n_top, uint32_t* top_id, float* top_logprob);
 /* Greedy generation after a prefill or forward: out_tokens[0] is the pending
  * pick, each of the next n_gen - 1 steps feeds the previous pick and picks
  * the next.  All on the device; returns when the tokens are on the host. */

@@ -112,6 +112,7 @@ SIGNATURES: dict[str, tuple] = {
     "m3g_decoder_upload": (ctypes.c_int, [_vp, _u32, _u32, _vp, _u64]),
     "m3g_decoder_forward": (ctypes.c_int, [_vp, _u32, _vp]),
     "m3g_decoder_prefill": (ctypes.c_int, [_vp, _vp, _u64, _vp]),
+    "m3g_decoder_score": (ctypes.c_int, [_vp, _vp, _u64, _vp, _vp, _u32, _vp, _vp]),
     "m3g_decoder_generate": (ctypes.c_int, [_vp, _u64, _vp]),
     "m3g_decoder_run_async": (ctypes.c_int, [_vp, _u64]),
     "m3g_decoder_sync": (ctypes.c_int, [_vp]),

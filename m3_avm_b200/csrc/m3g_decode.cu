@@ -432,6 +432,8 @@ struct m3g_decoder {
   bool p2p = false;
   bool shard_ffn = false;  // world > 1: FFN rows split too (else every rank keeps the layers, the head is split)
   uint8_t* peer_base[m3g::kMaxPeers] = {};
+  float* score = nullptr;  // results of m3g_decoder_score
+  size_t score_words = 0;
   int* h_io = nullptr;  // pinned: [0] token / nfixed staging, [1] last token
   uint32_t* status = nullptr;
   int pos = 0;           // host mirror of the device position
@@ -1087,6 +1089,51 @@ M3G_API int m3g_decoder_prefill(m3g_decoder* d, const uint32_t* tokens, uint64_t
   return check_status(d);
 }
 
+M3G_API int m3g_decoder_score(m3g_decoder* d, const uint32_t* tokens, uint64_t n, float* logprob, float* entropy,
+                              uint32_t n_top, uint32_t* top_id, float* top_logprob) {
+  if (!d || (!tokens && n) || (n_top && (!top_id || !top_logprob))) return host_fail(M3G_EINVAL, "null argument");
+  if (n_top > 32 || n_top > d->cfg.vocab)
+    return host_fail(M3G_EINVAL, "%u alternatives (at most 32, and the vocabulary)", n_top);
+  if (n == 0) return M3G_OK;
+  if (n > d->cfg.max_pos || d->pos + n > d->cfg.max_pos) return host_fail(M3G_EINVAL, "prompt overflows the KV cache");
+  for (uint64_t i = 0; i < n; ++i)
+    if (tokens[i] >= d->cfg.vocab) return host_fail(M3G_EINVAL, "token %u outside the vocabulary", tokens[i]);
+  DevGuard g(d->device);
+  DEC_CUDA(cudaStreamSynchronize(d->st));
+  const size_t words = n * (2 + 2 * static_cast<size_t>(n_top));
+  if (words > d->score_words) {
+    cudaFree(d->score);
+    d->score = nullptr;
+    d->score_words = 0;
+    DEC_CUDA(cudaMalloc(&d->score, 4 * words));
+    d->score_words = words;
+  }
+  float* lp = d->score;
+  float* ent = lp + n;
+  float* tops = ent + n;
+  int32_t* ids = reinterpret_cast<int32_t*>(tops + n * n_top);
+  const int first = d->pos, nfixed = first + static_cast<int>(n);
+  DEC_CUDA(cudaMemcpy(d->tokens + first, tokens, 4 * n, cudaMemcpyHostToDevice));
+  DEC_CUDA(cudaMemcpy(d->nfixed, &nfixed, 4, cudaMemcpyHostToDevice));
+  // A row is scored where the step left its logits: 10 us behind a step, which
+  // reads all weights; tokens[i + 1] is there by then, the last one's pick too.
+  for (uint64_t i = 0; i < n; ++i) {
+    if (int rc = run_steps(d, 1)) return rc;
+    if (int rc = gather_logits(d, true)) return rc;
+    if (int rc = m3g_token_logprobs_dev(M3G_DTYPE_F32, d->logits, 1, d->cfg.vocab, static_cast<int64_t>(d->cfg.vocab),
+                                        d->tokens + first + i + 1, 1, lp + i, ent + i, n_top, ids + i * n_top,
+                                        tops + i * n_top, d->st))
+      return rc;
+  }
+  if (logprob) DEC_CUDA(cudaMemcpyAsync(logprob, lp, 4 * n, cudaMemcpyDeviceToHost, d->st));
+  if (entropy) DEC_CUDA(cudaMemcpyAsync(entropy, ent, 4 * n, cudaMemcpyDeviceToHost, d->st));
+  if (n_top) {
+    DEC_CUDA(cudaMemcpyAsync(top_id, ids, 4 * n * n_top, cudaMemcpyDeviceToHost, d->st));
+    DEC_CUDA(cudaMemcpyAsync(top_logprob, tops, 4 * n * n_top, cudaMemcpyDeviceToHost, d->st));
+  }
+  return check_status(d);
+}
+
 M3G_API int m3g_decoder_generate(m3g_decoder* d, uint64_t n_gen, uint32_t* out_tokens) {
   if (!d || (!out_tokens && n_gen)) return host_fail(M3G_EINVAL, "null argument");
   if (n_gen == 0) return M3G_OK;
@@ -1182,7 +1229,7 @@ M3G_API void m3g_decoder_destroy(m3g_decoder* d) {
   for (void* p : {static_cast<void*>(d->xregion), static_cast<void*>(d->qkvb), static_cast<void*>(d->att),
                   static_cast<void*>(d->logits), static_cast<void*>(d->rope),
                   static_cast<void*>(d->kc), static_cast<void*>(d->vc), static_cast<void*>(d->dpos),
-                  static_cast<void*>(d->tokens)})
+                  static_cast<void*>(d->tokens), static_cast<void*>(d->score)})
     if (p) cudaFree(p);
   if (d->h_io) cudaFreeHost(d->h_io);
   if (d->st) cudaStreamDestroy(d->st);

@@ -15,6 +15,7 @@ import ctypes
 import numpy as np
 
 from . import _lib, model
+from .logprobs import TokenLogprobs
 
 
 class GpuDecoder:
@@ -85,6 +86,18 @@ class GpuDecoder:
             return np.zeros(self.shape.vocab, np.float32)
         _lib.check(_lib.load().m3g_decoder_prefill(self._h, t.ctypes.data, t.size, logits.ctypes.data))
         return logits
+
+    def score(self, tokens, n_top: int = 0) -> TokenLogprobs:
+        """prefill_logits(tokens) with, for each position i, the log probability of the token that follows it (tokens[i +
+        1]; for the last position the greedy pick), the entropy and the n_top <= 32 most probable ids there."""
+        t = np.ascontiguousarray(tokens, dtype=np.uint32)
+        lp, ent = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        ids = np.empty((t.size, n_top), np.uint32) if n_top > 0 else None
+        tops = np.empty((t.size, n_top), np.float32) if n_top > 0 else None
+        _lib.check(_lib.load().m3g_decoder_score(
+            self._h, t.ctypes.data, t.size, lp.ctypes.data, ent.ctypes.data, n_top,
+            ids.ctypes.data if n_top > 0 else None, tops.ctypes.data if n_top > 0 else None))
+        return TokenLogprobs(lp, ent, ids, tops)
 
     @staticmethod
     def sample(logits) -> int:

@@ -231,3 +231,7 @@ def test_python_checks_without_a_device():
                 dict(logits=x, tokens=i32(2)), dict(logits=x.double(), n_top=1), dict(logits=x, n_top=1)):
         with pytest.raises(M3GError):
             token_logprobs(**bad)
+
+
+def test_decoder_score_without_a_decoder(lib):
+    assert lib.m3g_decoder_score(None, None, 0, None, None, 0, None, None) == EINVAL
