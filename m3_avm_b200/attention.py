@@ -86,6 +86,12 @@ def _check_rows(name, t, device=None, heads=None, head_dim=None, tokens=None):
     return shape, strides
 
 
+def _check_sizes(what, *sizes):
+    """Sizes that the library takes as 32 bits (ctypes would cut them)."""
+    if min(sizes) < 0 or max(sizes) >= 2 ** 31:
+        _fail(f"size of the {what} out of range")
+
+
 def _check_ints(name, t, device, shape):
     if torch is None:
         _need_torch()
@@ -94,15 +100,18 @@ def _check_ints(name, t, device, shape):
 
 
 class Rope:
-    """A plan of rotary positions (m3g_rope_config); host arithmetic, usable on every device."""
+    """A plan of rotary positions (m3g_rope_config); host arithmetic, usable on every device.  Autograd does not see
+    the calls: the gradient of apply(...) is apply(..., inverse=True) of the results' gradients."""
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, theta: float = 10000.0, interleaved: bool = False,
                  scaling: str = "none", factor: float = 1.0, orig_ctx: int = 0, low_freq: float = 1.0,
                  high_freq: float = 4.0, beta_fast: float = 32.0, beta_slow: float = 1.0, magnitude: float = 0.0):
         if scaling not in SCALINGS:
             _fail(f"scaling {scaling!r}: one of {', '.join(SCALINGS)} is wanted")
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        _check_sizes("head", head_dim, rot_dim)
         self.head_dim = head_dim
-        cfg = _lib.RopeConfig(head_dim, rot_dim if rot_dim is not None else head_dim, 1 if interleaved else 0,
+        cfg = _lib.RopeConfig(head_dim, rot_dim, 1 if interleaved else 0,
                               SCALINGS[scaling], theta, factor, orig_ctx, low_freq, high_freq, beta_fast, beta_slow,
                               magnitude)
         h = ctypes.c_void_p()
@@ -158,8 +167,7 @@ class KvBatch:
         if page_table.dim() != 2:
             _fail("page_table: (sequences, pages) is wanted")
         _check_ints("page_table", page_table, self.device, (n, page_table.shape[1]))
-        if min(n_tokens, max_tokens, max_len) < 0:
-            _fail("negative size of the batch")
+        _check_sizes("batch", n_tokens, max_tokens, max_len)
         self.q_start, self.ctx_len, self.page_table = q_start, ctx_len, page_table
         self.n_tokens, self.max_tokens, self.max_len = n_tokens, max_tokens, max_len
         self.args = _lib.KvBatchArgs(q_start.data_ptr(), ctx_len.data_ptr(), page_table.data_ptr(), n,
@@ -174,8 +182,7 @@ class KvCache:
                  device: int = 0, pool=None):
         if torch is None:
             _need_torch()
-        if min(n_layers, n_kv_heads, head_dim, page_size, n_pages) < 0:
-            _fail("negative size of the cache")
+        _check_sizes("cache", n_layers, n_kv_heads, head_dim, page_size, n_pages)
         self.dtype, self.n_layers, self.n_kv_heads, self.head_dim = dtype, n_layers, n_kv_heads, head_dim
         self.page_size, self.n_pages = page_size, n_pages
         self.layout = _lib.KvLayout(dtype, n_layers, n_kv_heads, head_dim, page_size, n_pages)
@@ -233,8 +240,8 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
                    workspace=None, stream=None):
     """Attention of the batch's new tokens (already written) over the cache.  `mask`: int32 (tokens, words), bit i % 32
     of word i / 32 says whether the token sees new token i of its sequence; None: all up to and including itself.
-    `workspace`: a uint8 tensor of cache.attention_workspace(heads, q.dtype, batch.max_tokens) bytes, used by one call at a time (allocated here
-    when None)."""
+    `workspace`: a uint8 tensor of cache.attention_workspace(heads, q.dtype, batch.max_tokens) bytes, used by one call
+    at a time (allocated here when None)."""
     device, dtype = _device(q), act_dtype(q)
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
     heads = shape[1]
@@ -255,7 +262,8 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     if workspace is None:
         if stream is not None:
             _fail("a call on a stream of its own needs its own workspace")
-        workspace = torch.empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens), dtype=torch.uint8,
+                                device=q.device)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
     rq, ro = _lib.Rows(q.data_ptr(), sq[0], sq[1]), _lib.Rows(out.data_ptr(), so[0], so[1])

@@ -7,7 +7,8 @@
 // 0.06 rad at position 10^6).  sincospif of the top 32 bits gives cos and sin
 // once per token; all its heads share them through shared memory.
 //
-// Bound: HBM (each element read and written once).  A CTA takes a run of tokens.
+// Bound: HBM (each element read and written once; 16384 BF16 tokens of 72 heads of 128
+// 116 us, 5.2 TB/s; 4099 F32 tokens of 40 heads of 64 14.5 us, 5.8 TB/s).  A CTA takes a run of tokens.
 // Each thread copies its own pieces of the next kRopeDepth tokens into its own
 // places in shared memory (cp.async; nobody else reads them, so no barrier), so
 // that 3 x 64 bytes a thread are in flight without registers; the angles of as many tokens as there

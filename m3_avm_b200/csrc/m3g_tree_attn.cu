@@ -22,6 +22,16 @@
 // ring of stages filled by 16-byte cp.async; it keeps its own maximum, sum and
 // 16 x HD results in registers, so the warps meet only at the end of a piece.
 // The stages are swizzled so that the fragment loads touch all banks.
+//
+// Split.  The chunks of all sequences, heads and tiles form one line that the
+// CTAs cut evenly, whatever the lengths; a unit that is cut leaves its parts
+// (maximum, sum, results) in the workspace for k_tree_join.
+//
+// Bound.  With few rows HBM: 48 ragged contexts of up to 16000 positions, 4 rows
+// a KV head, BF16 over Q8_0: 245 us, 4.6 TB/s; the same loads without the
+// arithmetic take 181 us, the rest is ALU work (unpacking, softmax) beside them.
+// One context of 1024 positions: 9.3 us, of which a launch, the loads' latency
+// and the join each take 2 to 3.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

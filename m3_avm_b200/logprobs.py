@@ -22,8 +22,8 @@ def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, s
 
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _fail("logits: (rows, vocab) with a contiguous last dimension is wanted")
-    if n_top < 0:
-        _fail("n_top must not be negative")
+    if not 0 <= n_top <= 32:
+        _fail(f"{n_top} alternatives (at most 32)")
     rows, vocab = logits.shape
     device, dtype = _device(logits), act_dtype(logits)
     n, dev = 0, logits.device

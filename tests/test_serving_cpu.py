@@ -235,3 +235,21 @@ def test_python_checks_without_a_device():
 
 def test_decoder_score_without_a_decoder(lib):
     assert lib.m3g_decoder_score(None, None, 0, None, None, 0, None, None) == EINVAL
+
+
+def test_sizes_past_32_bits_are_refused():
+    from m3_avm_b200.attention import KvBatch, KvCache, Rope
+    from m3_avm_b200.logprobs import token_logprobs
+    import torch
+
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    for args in ((1, 1, 2 ** 32 + 16), (1, 2 ** 32 + 1, 16), (2 ** 32 + 1, 1, 16)):
+        with pytest.raises(M3GError):
+            KvBatch(i32(2), i32(1), i32(1, 4), *args)
+    for args in ((8, 2 ** 32 + 1, 2, 64, 16, 4), (8, 1, 2, 64, 2 ** 32 + 16, 4), (8, 1, 2, 2 ** 32 + 64, 16, 4)):
+        with pytest.raises(M3GError):
+            KvCache(*args, pool=torch.zeros(1 << 16, dtype=torch.uint8))
+    with pytest.raises(M3GError):
+        Rope(2 ** 32 + 64)
+    with pytest.raises(M3GError):
+        token_logprobs(torch.zeros(1, 4), n_top=2 ** 32 + 1)
