@@ -479,7 +479,8 @@ M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint3
  * [n_tokens][n_heads][head_dim] of `dtype`; `out` may be q itself.  Sums are
  * f32.  Products take the cached codes exactly and p as f16 (F32: q and p in
  * two f16 parts); large BF16 calls with more than 48 rows (tokens times query
- * heads per KV head) take the cached values, F16 ones V's, rounded to f16.
+ * heads per KV head) take the cached values rounded to f16, F16 ones V's (and
+ * p in two parts).
  * `workspace`: m3g_tree_attn_workspace() bytes (with the call's dtype, n_heads
  * and max_tokens) of device memory, 16-byte aligned, contents free, used by
  * one call at a time. */

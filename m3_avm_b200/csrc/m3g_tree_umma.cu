@@ -17,7 +17,9 @@
 //
 // Roundings.  Cached values enter as f16 products code * d (2^-11), or, for F16
 // activations, whose own step is as fine, K as two f16 parts (hi + lo, exact)
-// in two MMAs; weights as f16.  A group of 16 positions with a scale past 500 (a
+// in two MMAs and the weights as two (with one, a result was off by 1.6 times what
+// rounding it to f16 costs, with two 1.35 times, for 12 % of the time); otherwise
+// weights as f16.  A group of 16 positions with a scale past 500 (a
 // value could pass the f16 range) is taken at 2^-7, which its scores or weights
 // get back.
 //
@@ -28,7 +30,7 @@
 // and V's codes and scales (rows of a page are contiguous) two chunks ahead.
 // Measured: 8 trees of up to 64 tokens over contexts of up to 8190 (256 rows a KV
 // head, BF16 over Q8_0) 114 us, 12 trees of 13 over contexts of up to 30011 (104 rows,
-// F16 over Q4_0) 298 us.  Neither HBM nor the products bound it (their floors are
+// F16 over Q4_0) 333 us.  Neither HBM nor the products bound it (their floors are
 // 21 and 44 us): a chunk takes a CTA 3300 cycles of softmax and unpacking in
 // turn, a piece some 13000 to start, and waiting for instructions costs as much
 // as any other stall.
@@ -389,45 +391,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
         const int4 od = *reinterpret_cast<const int4*>(odd[ph & 3]);
         const int flags[4] = {od.x, od.y, od.z, od.w};
         const float lag = (od.x | od.y | od.z | od.w) & 2 ? kLagOddV : kLag;
-        // One pass takes the maximum and, with the reference so far, the weights;
-        // where a row's maximum grows past the lag they are taken again.
-        uint32_t p[32];
-        float sum;
-#pragma unroll 1
-        for (;;) {
-          const float ref = m == -INFINITY ? 0.f : m - kLift;
-          float mx = -INFINITY;
-          sum = 0.f;
-          uint32_t x[2][16];
-          tc_ld16_start(tl + buf * kUChunk, x[0]);
-#pragma unroll
-          for (int h = 0; h < kUChunk / 16; ++h) {
-            // a group at 2^-7: its scores, or its weights, get it back
-            const float csk = flags[h] & 1 ? 128.f * cs : cs, refv = flags[h] & 2 ? ref - 7.f : ref;
-            const uint64_t cs2 = pair(csk, csk), ref2 = pair(-refv, -refv);
-            uint32_t (&s)[16] = x[h & 1];
-            tc_ld_wait(s);
-            if (h + 1 < kUChunk / 16) tc_ld16_start(tl + buf * kUChunk + 16 * (h + 1), x[(h + 1) & 1]);
-            if (tail) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) s[j] = vis[h >> 1] >> (16 * (h & 1) + j) & 1u ? s[j] : 0xFF800000u;  // -inf
-            }
-            float top = -INFINITY;
-            uint64_t part = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float s0 = __uint_as_float(s[2 * j]), s1 = __uint_as_float(s[2 * j + 1]);
-              top = max3(top, s0, s1);
-              const uint64_t t = fma2(pair(s0, s1), cs2, ref2);
-              const float w0 = tex2(low(t)), w1 = tex2(high(t));
-              part = add2(part, pair(w0, w1));
-              p[8 * h + j] = pack_f16(w0, w1);
-            }
-            mx = fmaxf(mx, top * csk);
-            sum += (low(part) + high(part)) * (flags[h] & 2 ? 0x1p-7f : 1.f);
-          }
-          const bool grows = mx > m + lag || (m == -INFINITY && mx > -INFINITY);
-          if (!__any_sync(0xFFFFFFFFu, grows)) break;
+        auto rescale = [&](float mx, bool grows) {  // some row of the warp refers to a larger maximum from now on
           const float f = grows ? tex2(m - mx) : 1.f;
           if (grows) {
             m = mx;
@@ -445,9 +409,91 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
               tc_st16(tl + kOCol + 16 * h, x);
             }
           }
+        };
+        // The scores of a group of 16 positions, read while the one before is worked on.
+        uint32_t x[2][16];
+        auto scores = [&](int h) -> uint32_t(&)[16] {
+          uint32_t(&s)[16] = x[h & 1];
+          tc_ld_wait(s);
+          if (h + 1 < kUChunk / 16) tc_ld16_start(tl + buf * kUChunk + 16 * (h + 1), x[(h + 1) & 1]);
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = vis[h >> 1] >> (16 * (h & 1) + j) & 1u ? s[j] : 0xFF800000u;  // -inf
+          }
+          return s;
+        };
+        float sum = 0.f;
+        if constexpr (SPLIT) {  // the maximum first, then the weights, each group's in the place of its scores
+          float mx = -INFINITY;
+          tc_ld16_start(tl + buf * kUChunk, x[0]);
+#pragma unroll
+          for (int h = 0; h < kUChunk / 16; ++h) {
+            const uint32_t(&s)[16] = scores(h);
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) top = max3(top, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+            mx = fmaxf(mx, top * (flags[h] & 1 ? 128.f * cs : cs));
+          }
+          const bool grows = mx > m + lag || (m == -INFINITY && mx > -INFINITY);
+          if (__any_sync(0xFFFFFFFFu, grows)) rescale(mx, grows);
+          const float ref = m == -INFINITY ? 0.f : m - kLift;
+          tc_ld16_start(tl + buf * kUChunk, x[0]);
+#pragma unroll
+          for (int h = 0; h < kUChunk / 16; ++h) {
+            const float csk = flags[h] & 1 ? 128.f * cs : cs, refv = flags[h] & 2 ? ref - 7.f : ref;
+            const uint64_t cs2 = pair(csk, csk), ref2 = pair(-refv, -refv);
+            const uint32_t(&s)[16] = scores(h);
+            uint32_t p[16];
+            uint64_t part = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint64_t t = fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), cs2, ref2);
+              const float w0 = tex2(low(t)), w1 = tex2(high(t));
+              part = add2(part, pair(w0, w1));
+              p[j] = pack_f16(w0, w1);
+              const float2 hi = unpack_f16(p[j]);
+              p[8 + j] = pack_f16(w0 - hi.x, w1 - hi.y);
+            }
+            sum += (low(part) + high(part)) * (flags[h] & 2 ? 0x1p-7f : 1.f);
+            tc_st16(tl + buf * kUChunk + 16 * h, p);
+          }
+        } else {
+          // One pass takes the maximum and, with the reference so far, the weights;
+          // where a row's maximum grows past the lag they are taken again.
+          uint32_t p[32];
+#pragma unroll 1
+          for (;;) {
+            const float ref = m == -INFINITY ? 0.f : m - kLift;
+            float mx = -INFINITY;
+            sum = 0.f;
+            tc_ld16_start(tl + buf * kUChunk, x[0]);
+#pragma unroll
+            for (int h = 0; h < kUChunk / 16; ++h) {
+              // a group at 2^-7: its scores, or its weights, get it back
+              const float csk = flags[h] & 1 ? 128.f * cs : cs, refv = flags[h] & 2 ? ref - 7.f : ref;
+              const uint64_t cs2 = pair(csk, csk), ref2 = pair(-refv, -refv);
+              const uint32_t(&s)[16] = scores(h);
+              float top = -INFINITY;
+              uint64_t part = 0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float s0 = __uint_as_float(s[2 * j]), s1 = __uint_as_float(s[2 * j + 1]);
+                top = max3(top, s0, s1);
+                const uint64_t t = fma2(pair(s0, s1), cs2, ref2);
+                const float w0 = tex2(low(t)), w1 = tex2(high(t));
+                part = add2(part, pair(w0, w1));
+                p[8 * h + j] = pack_f16(w0, w1);
+              }
+              mx = fmaxf(mx, top * csk);
+              sum += (low(part) + high(part)) * (flags[h] & 2 ? 0x1p-7f : 1.f);
+            }
+            const bool grows = mx > m + lag || (m == -INFINITY && mx > -INFINITY);
+            if (!__any_sync(0xFFFFFFFFu, grows)) break;
+            rescale(mx, grows);
+          }
+          tc_st16(tl + buf * kUChunk, *reinterpret_cast<uint32_t(*)[16]>(&p[0]));
+          tc_st16(tl + buf * kUChunk + 16, *reinterpret_cast<uint32_t(*)[16]>(&p[16]));
         }
-        tc_st16(tl + buf * kUChunk, *reinterpret_cast<uint32_t(*)[16]>(&p[0]));
-        tc_st16(tl + buf * kUChunk + 16, *reinterpret_cast<uint32_t(*)[16]>(&p[16]));
         l += sum;
         if ((od.x | od.y | od.z | od.w) & 4) {
 #pragma unroll 1
@@ -627,8 +673,10 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kUChunk / 16; ++k)
-            tc_mma_ts(tbase + kOCol, tbase + buf * kUChunk + 8 * k, v0 + k * 256 / 16, idesc_f16(HD, true),
-                      c > 0 || k > 0);
+#pragma unroll
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+              tc_mma_ts(tbase + kOCol, tbase + buf * kUChunk + (SPLIT ? 16 : 8) * k + 8 * part, v0 + k * 256 / 16,
+                        idesc_f16(HD, true), c > 0 || k > 0 || part > 0);
           tc_commit(&bar.s_free[buf]);
           tc_commit(&bar.pv_done);
         }
