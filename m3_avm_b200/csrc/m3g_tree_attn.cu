@@ -547,17 +547,18 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool q8, int sms, cudaStream_t st) 
 }
 
 // Which form: the one of 128-row tiles (m3g_tree_umma.cu) for 16-bit types where a
-// KV head has more than 64 rows (48 for BF16 of 128 values, which needs no second
-// part of K) and there are 8 chunks for each of its CTAs.  Measured, that form
+// KV head has rows enough and there are 8 chunks for each of its CTAs.  F16 takes
+// more rows: K and the weights go into that form in two parts.  Measured, that form
 // against this one (32 query over 8 KV heads, Q8_0, 8 sequences of up to 8000
 // positions): BF16 of 128 values, 48 rows 75 against 71 us, 56 rows 76 against 78,
-// 256 rows 112 against 260; F16 of 128, 64 rows 93 against 88, 128 rows 100 against
-// 143; 64 values, 64 rows 57 against 55, 128 rows 61 against 90.  With fewer chunks
-// (2 sequences of 8000, 128 rows, 2000 chunks) 73 against 56 us; one sequence of
-// 2000 positions, 256 rows, 39 against 29.
+// 256 rows 112 against 260; of 64 values, 64 rows 57 against 55, 128 rows 61 against
+// 90; F16 of 128, 80 rows 100 against 94, 96 rows 102 against 116, 256 rows 155
+// against 260; of 64, 96 rows 72 against 70, 128 rows 75 against 89.  With fewer
+// chunks (BF16, 2 sequences of 8000, 128 rows, 2000 chunks) 73 against 56 us; one
+// sequence of 2000 positions, 256 rows, 39 against 29.
 constexpr uint64_t kUmmaChunks = 8 * 296;
 bool can_use_umma(const m3g_kv_layout* l, uint32_t dtype, uint32_t n_heads, uint32_t max_tokens) {
-  const uint64_t least = dtype == M3G_DTYPE_BF16 && l->head_dim == 128 ? 49 : 65;
+  const uint64_t least = dtype == M3G_DTYPE_F16 ? 81 : l->head_dim == 128 ? 49 : 65;
   return dtype != M3G_DTYPE_F32 && static_cast<uint64_t>(max_tokens) * (n_heads / l->n_kv_heads) >= least;
 }
 
