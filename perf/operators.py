@@ -177,7 +177,8 @@ def prepare(case, seed):
             from m3_avm_b200.attention import Rope
 
             s["plan"] = Rope(hd, rot_dim=case["rot_dim"], theta=case["theta"], interleaved=case["interleaved"],
-                             scaling=case["scaling"], factor=case["factor"], orig_ctx=8192)
+                             scaling=case["scaling"], factor=1.0 if case["scaling"] == "none" else case["factor"],
+                             orig_ctx=8192)
         return s
     ctx, new = _lengths(case)
     page, n = case["page"], case["seqs"]
