@@ -86,6 +86,11 @@ def _check_rows(name, t, device=None, heads=None, head_dim=None, tokens=None):
     return shape, strides
 
 
+def _new_like(t):
+    """An uninitialised contiguous tensor of t's shape and type (empty_like takes two thirds of new_empty's time)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _check_sizes(what, *sizes):
     """Sizes that the library takes as 32 bits (ctypes would cut them)."""
     if min(sizes) < 0 or max(sizes) >= 2 ** 31:
@@ -131,12 +136,14 @@ class Rope:
                 results.append(None)
                 continue
             shape, sx = _check_rows(name, x, device, None, self.head_dim, n)
+            heads = shape[1]
             if y is None:
-                y = x.new_empty(shape)
-            shape, sy = _check_rows(name + "_out", y, device, shape[1], self.head_dim, n)
+                y, sy = _new_like(x), (heads * self.head_dim, self.head_dim)
+            else:
+                _, sy = _check_rows(name + "_out", y, device, heads, self.head_dim, n)
             if x.dtype is not q.dtype or y.dtype is not q.dtype:
                 _fail("q, k and their results have one type")
-            args.append(_lib.RopeRows(x.data_ptr(), y.data_ptr(), shape[1], sx[0], sx[1], sy[0], sy[1]))
+            args.append(_lib.RopeRows(x.data_ptr(), y.data_ptr(), heads, sx[0], sx[1], sy[0], sy[1]))
             results.append(y)
         _call(_lib.load().m3g_rope_dev, device, stream, self._h, dtype, positions.data_ptr(), n, ctypes.byref(args[0]),
               ctypes.byref(args[1]) if args[1] is not None else None, 1 if inverse else 0)
@@ -219,7 +226,7 @@ class KvCache:
         if k_out is None:
             k_out = torch.empty(shape, dtype=dtype or torch.float32, device=self.pool.device)
         if v_out is None:
-            v_out = torch.empty(shape, dtype=k_out.dtype, device=self.pool.device)
+            v_out = _new_like(k_out)
         self._io(_lib.load().m3g_kv_read_dev, layer, k_out, v_out, batch, stream)
         return k_out, v_out
 
@@ -246,10 +253,11 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
     heads = shape[1]
     if out is None:
-        out = q.new_empty(shape)
-    elif out.dtype is not q.dtype:
-        _fail("q and out have one type")
-    _, so = _check_rows("out", out, device, heads, cache.head_dim, batch.n_tokens)
+        out, so = _new_like(q), (heads * cache.head_dim, cache.head_dim)
+    else:
+        if out.dtype is not q.dtype:
+            _fail("q and out have one type")
+        _, so = _check_rows("out", out, device, heads, cache.head_dim, batch.n_tokens)
     if batch.device != device:
         _fail("the batch is on another device than q")
     words, bits = 0, None
@@ -262,8 +270,7 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     if workspace is None:
         if stream is not None:
             _fail("a call on a stream of its own needs its own workspace")
-        workspace = torch.empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens), dtype=torch.uint8,
-                                device=q.device)
+        workspace = cache.pool.new_empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens))
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
     rq, ro = _lib.Rows(q.data_ptr(), sq[0], sq[1]), _lib.Rows(out.data_ptr(), so[0], so[1])

@@ -31,12 +31,12 @@ def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, s
     if tokens is not None:
         n = tokens.shape[-1] if tokens.dim() == 2 else -1
         _check_ints("tokens", tokens, device, (rows, n))
-        lp = logits.new_empty((rows, n), dtype=torch.float32)
+        lp = torch.empty_like(tokens, dtype=torch.float32)
     if entropy:
         ent = logits.new_empty((rows,), dtype=torch.float32)
     if n_top:
         ids = logits.new_empty((rows, n_top), dtype=torch.int32)
-        tops = logits.new_empty((rows, n_top), dtype=torch.float32)
+        tops = torch.empty_like(ids, dtype=torch.float32)
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     _call(_lib.load().m3g_token_logprobs_dev, device, stream, dtype, logits.data_ptr(), rows, vocab, logits.stride(0),
           ptr(tokens), n, ptr(lp), ptr(ent), n_top, ptr(ids), ptr(tops))
