@@ -250,17 +250,17 @@ __device__ __noinline__ LpSum lp_extreme(const T* x, long long e0, long long e1,
   return s;
 }
 
-// The first n of 16 bytes of logits, -inf behind them.
+// Logits lo .. hi-1 of 16 bytes of them, -inf for the others.
 template <class T>
-__device__ __noinline__ uint4 lp_tail(const T* x, int n) {
+__device__ __noinline__ uint4 lp_part(const T* x, int lo, int hi) {
   constexpr int VW = 16 / sizeof(T);
   __align__(16) T t[VW];
 #pragma unroll
-  for (int k = 0; k < VW; ++k) t[k] = k < n ? x[k] : Act<T>::from(-INFINITY);
+  for (int k = 0; k < VW; ++k) t[k] = k >= lo && k < hi ? x[k] : Act<T>::from(-INFINITY);
   return *reinterpret_cast<const uint4*>(t);
 }
 
-template <class T, bool VEC, bool TOP>
+template <class T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_constant__ LpArgs a) {
   constexpr int VW = 16 / sizeof(T), E = kLpVecs * VW, kRound = kLpThreads * E;
   __shared__ unsigned long long list[TOP ? kLpList : 1];
@@ -276,16 +276,22 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long row = blockIdx.x / size;
   const T* x = static_cast<const T*>(a.x) + row * a.stride;
+  // Elements are counted from the 16-byte boundary at or before the row: `lead` are not the row's.
+  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+  const T* base = x - lead;
   const long long e0 = static_cast<long long>(rank) * a.chunk;
-  const long long e1 = min(a.vocab, e0 + a.chunk);
+  const long long e1 = min(a.vocab + lead, e0 + a.chunk);
+  const long long own0 = max(e0 - lead, 0ll), own1 = e1 - lead;  // the CTA's logits
   union Raw {  // a round's logits of this thread
     uint4 q[kLpVecs];
     T t[E];
     __device__ Raw() {}
   };
+  uint4 none;  // -inf throughout
+  none.x = none.y = none.z = none.w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
   auto fetch = [&](long long r0, Raw& w) {
-    if (VEC && r0 + kRound <= e1) {
-      const uint4* p = reinterpret_cast<const uint4*>(x + r0) + tid;
+    if (r0 >= lead && r0 + kRound <= e1) {
+      const uint4* p = reinterpret_cast<const uint4*>(base + r0) + tid;
 #pragma unroll
       for (int j = 0; j < kLpVecs; ++j) w.q[j] = __ldcs(p + j * kLpThreads);
       return;
@@ -293,13 +299,18 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
 #pragma unroll
     for (int j = 0; j < kLpVecs; ++j) {
       const long long i = r0 + (j * kLpThreads + tid) * VW;
-      if (VEC && i + VW <= e1) w.q[j] = __ldcs(reinterpret_cast<const uint4*>(x + i));
-      else w.q[j] = lp_tail(x + i, static_cast<int>(min(e1 - i, static_cast<long long>(VW))));
+      if (i >= lead && i + VW <= e1) w.q[j] = __ldcs(reinterpret_cast<const uint4*>(base + i));
+      else if (i >= e1) w.q[j] = none;
+      else w.q[j] = lp_part(base + i, static_cast<int>(max(lead - i, 0ll)), static_cast<int>(min(e1 - i, static_cast<long long>(VW))));
     }
   };
   LpSum s{-INFINITY, 0.f, 0.f};
   float run = -INFINITY, bound = -INFINITY;
   bool again = true;  // the bound is to be raised
+  // Lanes to a group whose maximum counts for the bound: a half-warp, fewer where a
+  // short row leaves threads without logits, so that 32 groups have some.
+  int group = 16;
+  while (group > 1 && e1 - e0 <= 16ll * group * VW) group >>= 1;
   auto use = [&](long long r0, const Raw& w) {
     const float most = largest<T, E>(w.t);
     const float t_most = fmaxf(most, Lp<T>::kLow) * kLog2e;
@@ -339,9 +350,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
       run = fmaxf(run, most);
       if (again) {  // this warp's maxima into the shared ones, the bound from all of them
         float g = run;
-#pragma unroll
-        for (int o = 8; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-        if ((lane & 15) == 0) *const_cast<volatile float*>(&group_max[2 * warp + (lane >> 4)]) = g;
+        for (int o = group >> 1; o; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
+        if ((lane & (group - 1)) == 0 && tid < 32 * group) *const_cast<volatile float*>(&group_max[tid / group]) = g;
         if (r0 == e0) __syncthreads();
         else __syncwarp();
         bound = kth_of_lanes(*const_cast<volatile float*>(&group_max[lane]), a.n_top);
@@ -385,14 +395,14 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
     if (lane == 0) total = s;
   }
   if (TOP) {
-    const int most = static_cast<int>(min(static_cast<long long>(a.n_top), e1 - e0));
+    const int most = static_cast<int>(min(static_cast<long long>(a.n_top), own1 - own0));
     const int kept = n_copies;
     for (int c = warp; c < min(kept, kLpCopies); c += kLpThreads / 32) {
       if (lane < E) {
         const float v = Act<T>::to(reinterpret_cast<const T*>(copies[c])[lane]);
         if (v >= bound && v > -INFINITY) {
           const int at = atomicAdd(&count, 1), round = copy_of[c] / kLpThreads, thread = copy_of[c] % kLpThreads;
-          const long long i = e0 + static_cast<long long>(round) * kRound + (lane / VW * kLpThreads + thread) * VW + lane % VW;
+          const long long i = e0 - lead + static_cast<long long>(round) * kRound + (lane / VW * kLpThreads + thread) * VW + lane % VW;
           if (at < kLpList) list[at] = lp_key(v, static_cast<uint32_t>(i));
         }
       }
@@ -401,7 +411,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
     const int n = count;
     int got;
     if (kept > kLpCopies || n > kLpList || n < most) {
-      got = lp_walk(x, e0, e1, a.n_top, list, best, red, &count);
+      got = lp_walk(x, own0, own1, a.n_top, list, best, red, &count);
     } else {
       lp_select(list, n, a.n_top, best, red);
       got = min(n, a.n_top);
@@ -414,7 +424,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
   if (size > 1) all = join_lanes(lane < size ? *cluster.map_shared_rank(&total, lane) : LpSum{-INFINITY, 0.f, 0.f}, 32);
   const bool extreme = !(all.m > Lp<T>::kRowLow * kLog2e && all.m < 1e38f * kLog2e);  // the same in the whole cluster
   if (extreme) {
-    const LpSum mine = lp_extreme(x, e0, e1, sums);
+    const LpSum mine = lp_extreme(x, own0, own1, sums);
     if (tid == 0) coarse = mine;
     if (size > 1) cluster.sync();
     else __syncthreads();
@@ -454,7 +464,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) k_token_logprobs(const __grid_c
   if (size > 1) cluster.sync();  // the others' shared memory stays until rank 0 has read it
 }
 
-template <class T, bool VEC, bool TOP>
+template <class T, bool TOP>
 cudaError_t launch_lp(const LpArgs& a, long long rows, int cluster, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
@@ -468,15 +478,14 @@ cudaError_t launch_lp(const LpArgs& a, long long rows, int cluster, cudaStream_t
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_token_logprobs<T, VEC, TOP>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_token_logprobs<T, TOP>, a);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
 
 template <class T>
-cudaError_t launch_lp_t(const LpArgs& a, long long rows, bool vec, int cluster, cudaStream_t st) {
-  if (a.n_top) return vec ? launch_lp<T, true, true>(a, rows, cluster, st) : launch_lp<T, false, true>(a, rows, cluster, st);
-  return vec ? launch_lp<T, true, false>(a, rows, cluster, st) : launch_lp<T, false, false>(a, rows, cluster, st);
+cudaError_t launch_lp_t(const LpArgs& a, long long rows, int cluster, cudaStream_t st) {
+  return a.n_top ? launch_lp<T, true>(a, rows, cluster, st) : launch_lp<T, false>(a, rows, cluster, st);
 }
 
 }  // namespace
@@ -501,6 +510,7 @@ M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t 
   if (!rows) return M3G_OK;
   if (!logits || (n_tokens && (!tokens || !logprob)) || (n_top && (!top_id || !top_logprob)))
     return host_fail(M3G_EINVAL, "null argument");
+  if (reinterpret_cast<uintptr_t>(logits) % size) return host_fail(M3G_EINVAL, "logits not aligned to their type");
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
   int cluster = 1;
@@ -516,13 +526,12 @@ M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t 
   a.top_lp = top_logprob;
   a.n_tokens = static_cast<int>(n_tokens);
   a.n_top = static_cast<int>(n_top);
-  a.chunk = static_cast<int>((vocab + cluster - 1) / cluster + 15) / 16 * 16;
-  const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride * size % 16 == 0;
+  a.chunk = static_cast<int>((vocab + 7 + cluster - 1) / cluster + 15) / 16 * 16;  // 7: the most a row starts behind a boundary
   const cudaStream_t st = serve_stream(stream);
   const long long n = static_cast<long long>(rows);
-  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_lp_t<float>(a, n, vec, cluster, st)
-                        : dtype == M3G_DTYPE_F16 ? launch_lp_t<__half>(a, n, vec, cluster, st)
-                                                 : launch_lp_t<__nv_bfloat16>(a, n, vec, cluster, st);
+  const cudaError_t e = dtype == M3G_DTYPE_F32   ? launch_lp_t<float>(a, n, cluster, st)
+                        : dtype == M3G_DTYPE_F16 ? launch_lp_t<__half>(a, n, cluster, st)
+                                                 : launch_lp_t<__nv_bfloat16>(a, n, cluster, st);
   if (e != cudaSuccess) return host_fail(M3G_ECUDA, "k_token_logprobs: %s", cudaGetErrorString(e));
   return M3G_OK;
 }
