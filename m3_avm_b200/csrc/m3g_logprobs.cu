@@ -26,12 +26,12 @@
 // but the largest have a probability of 0.
 //
 // A row is read by a cluster of 1 .. 8 CTAs, whose sums and lists join through
-// distributed shared memory: 8 while the rows do not fill the SMs.
+// distributed shared memory: as many as leave no SM with two.
 //
-// Measured: 1031 BF16 rows of 128256 with 5 alternatives 65 us (4.1 TB/s; without
+// Measured: 1031 BF16 rows of 128256 with 5 alternatives 66 us (4.0 TB/s; without
 // alternatives 53).  The exponentials, 16 a cycle and SM, take 36 us by themselves,
 // the rest of the loop about as many issue slots; reading takes 41.  One F32 row
-// with 20 alternatives 10 us: launch, two loads' latency and the joins in turn.
+// with 20 alternatives 11 us: launch, two loads' latency and the joins in turn.
 #include <cmath>
 #include <type_traits>
 
@@ -513,8 +513,11 @@ M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t 
   if (reinterpret_cast<uintptr_t>(logits) % size) return host_fail(M3G_EINVAL, "logits not aligned to their type");
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
+  // As many CTAs to a row as the SMs hold one each of: clusters that come in a
+  // second wave wait for whole ones to end (74 rows of 128256 BF16, 20 alternatives:
+  // 15 us with 148 CTAs, 35 with 592; 148 rows 17 us with one CTA each, 35 with four).
   int cluster = 1;
-  while (cluster < 8 && rows * cluster * 2 <= 592 && vocab / (cluster * 2) >= 4096) cluster *= 2;
+  while (cluster < 8 && rows * cluster * 2 <= 148 && vocab / (cluster * 2) >= 4096) cluster *= 2;
   LpArgs a{};
   a.x = logits;
   a.vocab = static_cast<long long>(vocab);

@@ -253,3 +253,10 @@ def test_sizes_past_32_bits_are_refused():
         Rope(2 ** 32 + 64)
     with pytest.raises(M3GError):
         token_logprobs(torch.zeros(1, 4), n_top=2 ** 32 + 1)
+
+
+def test_logits_off_their_types_alignment_are_refused(lib):
+    buf = (ctypes.c_uint8 * 64)()
+    at = ctypes.addressof(buf) // 16 * 16 + 16
+    for dtype, off in ((0, 2), (1, 1), (30, 1)):
+        assert lib.m3g_token_logprobs_dev(dtype, at + off, 1, 4, 4, None, 0, None, at, 0, None, None, None) == EINVAL
