@@ -376,7 +376,8 @@ M3G_API int m3g_matvec_greedy_noalloc(const float* x, const uint8_t* raw, uint64
  * in the reference, whose forward_one (src/inference.rs:953-1152) advances one
  * sequence by one token over an f32 cache.  Activations are F32, F16 or BF16
  * device memory (`dtype` of each call); the last dimension is contiguous, the
- * other strides are in elements and free (not negative).  Calls hold no state:
+ * other strides are in elements and free (not negative); pointers are multiples
+ * of their elements' size (M3G_EINVAL otherwise).  Calls hold no state:
  * any number may run at once on different streams, and all can be captured. */
 
 /* Rotary positions.  Pair i of a head, (x[i], x[i + rot_dim/2]), or (x[2i],

@@ -49,6 +49,8 @@ int kv_batch_check(const m3g_kv_layout* l, const m3g_kv_batch* b) {
     return host_fail(M3G_EINVAL, "batch too large");
   if (b->n_seqs && b->n_tokens && (!b->q_start || !b->ctx_len || !b->page_table || !b->max_pages))
     return host_fail(M3G_EINVAL, "null batch array");
+  if (misaligned(b->q_start, 4) || misaligned(b->ctx_len, 4) || misaligned(b->page_table, 4))
+    return host_fail(M3G_EINVAL, "batch array not 4-byte aligned");
   (void)l;
   return M3G_OK;
 }
@@ -424,6 +426,7 @@ int kv_io(const m3g_kv_layout* l, const void* pool, uint32_t layer, const m3g_kv
   bool vec = true;
   for (const m3g_rows* r : {k, v}) {
     if (!r->p && b->n_tokens) return host_fail(M3G_EINVAL, "null rows");
+    if (misaligned(r->p, size)) return host_fail(M3G_EINVAL, "rows not aligned to their type");
     if (r->token_stride < 0 || r->head_stride < 0) return host_fail(M3G_EINVAL, "negative stride");
     if (!write && ((b->n_tokens > 1 && r->token_stride < a.p.hd) || (a.p.kvh > 1 && r->head_stride < a.p.hd)))
       return host_fail(M3G_EINVAL, "result rows overlap");

@@ -510,7 +510,11 @@ M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t 
   if (!rows) return M3G_OK;
   if (!logits || (n_tokens && (!tokens || !logprob)) || (n_top && (!top_id || !top_logprob)))
     return host_fail(M3G_EINVAL, "null argument");
-  if (reinterpret_cast<uintptr_t>(logits) % size) return host_fail(M3G_EINVAL, "logits not aligned to their type");
+  if (misaligned(logits, size)) return host_fail(M3G_EINVAL, "logits not aligned to their type");
+  for (const void* p : {static_cast<const void*>(tokens), static_cast<const void*>(logprob),
+                        static_cast<const void*>(entropy), static_cast<const void*>(top_id),
+                        static_cast<const void*>(top_logprob)})
+    if (misaligned(p, 4)) return host_fail(M3G_EINVAL, "tokens or results not 4-byte aligned");
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
   // As many CTAs to a row as the SMs hold one each of: clusters that come in a

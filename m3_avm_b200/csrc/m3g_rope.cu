@@ -326,6 +326,8 @@ M3G_API int m3g_rope_dev(const m3g_rope* rope, uint32_t dtype, const int32_t* po
     const m3g_rope_rows& r = i ? *k : *q;
     if (r.heads > (1u << 20)) return host_fail(M3G_EINVAL, "too many heads");
     if (r.heads && n_tokens && (!r.x || !r.y)) return host_fail(M3G_EINVAL, "null rows");
+    if (m3g::misaligned(r.x, size) || m3g::misaligned(r.y, size))
+      return host_fail(M3G_EINVAL, "rows not aligned to their type");
     if (r.x_token_stride < 0 || r.x_head_stride < 0 || r.y_token_stride < 0 || r.y_head_stride < 0)
       return host_fail(M3G_EINVAL, "negative stride");
     if (r.x == r.y && (r.x_token_stride != r.y_token_stride || r.x_head_stride != r.y_head_stride))
@@ -338,7 +340,7 @@ M3G_API int m3g_rope_dev(const m3g_rope* rope, uint32_t dtype, const int32_t* po
     heads += r.heads;
   }
   if (!n_tokens || !heads) return M3G_OK;
-  if (!positions) return host_fail(M3G_EINVAL, "null positions");
+  if (!positions || m3g::misaligned(positions, 4)) return host_fail(M3G_EINVAL, "positions null or not 4-byte aligned");
   a.positions = positions;
   a.heads = static_cast<int>(heads);
   a.heads0 = static_cast<int>(q->heads);

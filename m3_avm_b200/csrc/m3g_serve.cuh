@@ -125,6 +125,9 @@ inline bool rows_aligned(const void* p, int64_t token_stride, int64_t head_strid
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && token_stride * size % 16 == 0 && head_stride * size % 16 == 0;
 }
 
+// A pointer that is not a multiple of its elements' size (an access would fault).
+inline bool misaligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
+
 // The current device and its status word.
 inline int serve_device(int* dev, uint32_t** status) {
   if (cudaGetDevice(dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");

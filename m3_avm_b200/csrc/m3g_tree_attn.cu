@@ -599,6 +599,7 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   if (!size) return host_fail(M3G_EINVAL, "attention of dtype %u (F32, F16 and BF16 are supported)", dtype);
   for (const m3g_rows* r : {q, out}) {
     if (!r->p && b->n_tokens) return host_fail(M3G_EINVAL, "null rows");
+    if (misaligned(r->p, size)) return host_fail(M3G_EINVAL, "rows not aligned to their type");
     if (r->token_stride < 0 || r->head_stride < 0) return host_fail(M3G_EINVAL, "negative stride");
   }
   if ((b->n_tokens > 1 && out->token_stride < a.p.hd) || (n_heads > 1 && out->head_stride < a.p.hd))
@@ -606,6 +607,7 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   if (q->p == out->p && (q->token_stride != out->token_stride || q->head_stride != out->head_stride))
     return host_fail(M3G_EINVAL, "results in place of q need the same strides");
   if (!std::isfinite(scale) || scale < 0.f) return host_fail(M3G_EINVAL, "scale must be finite and not negative");
+  if (misaligned(mask, 4)) return host_fail(M3G_EINVAL, "mask not 4-byte aligned");
   if (mask && static_cast<uint64_t>(mask_words) * 32 < b->max_tokens)
     return host_fail(M3G_EINVAL, "%u mask words for %u tokens", mask_words, b->max_tokens);
   uint64_t need = 0;

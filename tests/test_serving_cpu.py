@@ -255,6 +255,23 @@ def test_sizes_past_32_bits_are_refused():
         token_logprobs(torch.zeros(1, 4), n_top=2 ** 32 + 1)
 
 
+def test_pointers_off_their_types_alignment_are_refused(lib):
+    write, attn, p, _keep = _calls(lib)
+    for f in (write, lambda **kw: write(read=True, **kw), attn):
+        assert f(a=(p + 2, 512, 128)) == EINVAL
+        assert f(b=(p + 8193, 512, 128), dtype=30) == EINVAL
+        for name in ("q_start", "ctx_len", "page_table"):
+            assert f(batch={name: p + 2}) == EINVAL
+    assert attn(mask=p + 2, words=1) == EINVAL
+    h = ctypes.c_void_p()
+    cfg = _lib.RopeConfig(64, 64, 0, 0, 10000.0, 1.0, 0, 1.0, 4.0, 32.0, 1.0, 0.0)
+    assert lib.m3g_rope_create(ctypes.byref(cfg), ctypes.byref(h)) == 0
+    for x, y, pos, dtype in ((p + 2, p + 4096, p, 0), (p, p + 4097, p, 1), (p, p + 4096, p + 1, 30)):
+        rows = _lib.RopeRows(x, y, 2, 128, 64, 128, 64)
+        assert lib.m3g_rope_dev(h, dtype, pos, 4, ctypes.byref(rows), None, 0, None) == EINVAL
+    lib.m3g_rope_destroy(h)
+
+
 def test_logits_off_their_types_alignment_are_refused(lib):
     buf = (ctypes.c_uint8 * 64)()
     at = ctypes.addressof(buf) // 16 * 16 + 16
