@@ -5,9 +5,12 @@ A step of a batch: ``Rope.apply`` turns q and k, ``KvCache.write`` puts the new
 tokens' K and V into the cache, ``tree_attention`` attends over it; ``KvBatch``
 says which tokens belong to which sequence.  Tensors are f32, f16 or bf16 of
 shape (tokens, heads, head_dim), any strides with a contiguous last dimension.
-Everything runs on `stream` (the current one of the tensors' device by
-default), enqueued without waiting, and raises M3GError for what the library
-refuses.
+Everything runs on `stream` (a raw handle; the current one of the tensors'
+device by default), enqueued without waiting, and raises M3GError for what the
+library refuses.  Given another stream than the current one, a call expects
+its inputs to be ready there; results and workspaces that it allocates are
+that stream's memory, kept until the current stream's work on them is done
+too, and whoever reads them elsewhere waits for the stream first.
 """
 from __future__ import annotations
 
@@ -91,6 +94,19 @@ def _new_like(t):
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
+def _on(device, stream, make, /, *args, **kw):
+    """make(*args, **kw), a new tensor, for a call on `stream`.  The allocator takes it that a block is used on the stream
+    that was current when it was handed out: a result made under another one could share its memory with that stream's
+    pending work, or be handed out again before the call has written it."""
+    if stream is None or stream == _current_stream(device):
+        return make(*args, **kw)
+    own = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(own):
+        t = make(*args, **kw)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
 def _check_sizes(what, *sizes):
     """Sizes that the library takes as 32 bits (ctypes would cut them)."""
     if min(sizes) < 0 or max(sizes) >= 2 ** 31:
@@ -138,7 +154,7 @@ class Rope:
             shape, sx = _check_rows(name, x, device, None, self.head_dim, n)
             heads = shape[1]
             if y is None:
-                y, sy = _new_like(x), (heads * self.head_dim, self.head_dim)
+                y, sy = _on(device, stream, _new_like, x), (heads * self.head_dim, self.head_dim)
             else:
                 _, sy = _check_rows(name + "_out", y, device, heads, self.head_dim, n)
             if x.dtype is not q.dtype or y.dtype is not q.dtype:
@@ -222,11 +238,11 @@ class KvCache:
 
     def read(self, layer: int, batch: KvBatch, dtype=None, k_out=None, v_out=None, stream=None):
         """The values held at the new tokens' places, as (k, v) of `dtype` (f32 by default)."""
-        shape = (batch.n_tokens, self.n_kv_heads, self.head_dim)
+        device, shape = _device(self.pool), (batch.n_tokens, self.n_kv_heads, self.head_dim)
         if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype or torch.float32, device=self.pool.device)
+            k_out = _on(device, stream, torch.empty, shape, dtype=dtype or torch.float32, device=self.pool.device)
         if v_out is None:
-            v_out = _new_like(k_out)
+            v_out = _on(device, stream, _new_like, k_out)
         self._io(_lib.load().m3g_kv_read_dev, layer, k_out, v_out, batch, stream)
         return k_out, v_out
 
@@ -253,7 +269,7 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
     heads = shape[1]
     if out is None:
-        out, so = _new_like(q), (heads * cache.head_dim, cache.head_dim)
+        out, so = _on(device, stream, _new_like, q), (heads * cache.head_dim, cache.head_dim)
     else:
         if out.dtype is not q.dtype:
             _fail("q and out have one type")
@@ -268,9 +284,8 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     if scale is not None and not scale > 0:
         _fail("scale must be positive")
     if workspace is None:
-        if stream is not None:
-            _fail("a call on a stream of its own needs its own workspace")
-        workspace = cache.pool.new_empty(cache.attention_workspace(heads, q.dtype, batch.max_tokens))
+        workspace = _on(device, stream, cache.pool.new_empty,
+                        cache.attention_workspace(heads, q.dtype, batch.max_tokens))
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _fail("workspace: a contiguous uint8 tensor on q's device is wanted")
     rq, ro = _lib.Rows(q.data_ptr(), sq[0], sq[1]), _lib.Rows(out.data_ptr(), so[0], so[1])

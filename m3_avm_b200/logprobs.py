@@ -5,7 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from . import _lib
-from .attention import _call, _check_ints, _device, _fail, act_dtype
+from .attention import _call, _check_ints, _device, _fail, _on, act_dtype
 
 
 class TokenLogprobs(NamedTuple):
@@ -17,7 +17,8 @@ class TokenLogprobs(NamedTuple):
 
 def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, stream=None) -> TokenLogprobs:
     """logits (rows, vocab) f32, f16 or bf16 with a contiguous last dimension; tokens int32 (rows, n) ids whose log
-    probabilities are wanted (-inf for an id outside the vocabulary); n_top <= 32 most probable ids of each row."""
+    probabilities are wanted (-inf for an id outside the vocabulary), at most 512 a row; n_top <= 32 most probable ids
+    of each row.  `stream` as in m3_avm_b200.attention."""
     import torch
 
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -26,17 +27,17 @@ def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, s
         _fail(f"{n_top} alternatives (at most 32)")
     rows, vocab = logits.shape
     device, dtype = _device(logits), act_dtype(logits)
-    n, dev = 0, logits.device
+    n = 0
     lp = ent = ids = tops = None
     if tokens is not None:
         n = tokens.shape[-1] if tokens.dim() == 2 else -1
         _check_ints("tokens", tokens, device, (rows, n))
-        lp = torch.empty_like(tokens, dtype=torch.float32)
+        lp = _on(device, stream, torch.empty_like, tokens, dtype=torch.float32)
     if entropy:
-        ent = logits.new_empty((rows,), dtype=torch.float32)
+        ent = _on(device, stream, logits.new_empty, (rows,), dtype=torch.float32)
     if n_top:
-        ids = logits.new_empty((rows, n_top), dtype=torch.int32)
-        tops = torch.empty_like(ids, dtype=torch.float32)
+        ids = _on(device, stream, logits.new_empty, (rows, n_top), dtype=torch.int32)
+        tops = _on(device, stream, torch.empty_like, ids, dtype=torch.float32)
     ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
     _call(_lib.load().m3g_token_logprobs_dev, device, stream, dtype, logits.data_ptr(), rows, vocab, logits.stride(0),
           ptr(tokens), n, ptr(lp), ptr(ent), n_top, ptr(ids), ptr(tops))

@@ -1,0 +1,79 @@
+"""Edges of the serving operators that need no GPU: whose memory results are, and what is refused."""
+import contextlib
+
+import pytest
+import torch
+
+from m3_avm_b200 import attention as A
+from m3_avm_b200 import logprobs as L
+
+
+def i32(*s):
+    return torch.zeros(s, dtype=torch.int32)
+
+
+# ---------------------------------------------------------------- results of a call on another stream
+class Streams:
+    """Stands in for the device: the current stream is 0, launches do nothing, allocations say where they were made."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.made, self.kept, self.launched = 0, [], [], []
+        for name in ("empty", "empty_like"):
+            monkeypatch.setattr(torch, name, self._noted(getattr(torch, name)))
+        new_empty = torch.Tensor.new_empty
+        monkeypatch.setattr(torch.Tensor, "new_empty", self._noted(new_empty))
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda stream, device=None: stream)
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: 0)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.current)
+        monkeypatch.setattr(torch.cuda, "stream", self._on)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: self.kept.append((t.data_ptr(), s)))
+        A._need_torch()
+        monkeypatch.setattr(A, "_need_torch", lambda: None)
+        monkeypatch.setattr(A, "_current_stream", lambda device: 0)
+        for module in (A, L):
+            monkeypatch.setattr(module, "_device", lambda t: -1)
+            monkeypatch.setattr(module, "_call", lambda fn, device, stream, *args: self.launched.append(stream))
+
+    def _noted(self, make):
+        def run(*args, **kw):
+            t = make(*args, **kw)
+            self.made.append((t.data_ptr(), self.current))
+            return t
+        return run
+
+    @contextlib.contextmanager
+    def _on(self, stream):
+        before, self.current = self.current, stream
+        yield
+        self.current = before
+
+
+def calls():
+    q, k = torch.randn(3, 4, 64), torch.randn(3, 2, 64)
+    cache = A.KvCache(8, 1, 2, 64, 16, 4, pool=torch.zeros(4 * 2 * 16 * 2 * 68, dtype=torch.uint8))
+    batch = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64)
+    x = torch.randn(3, 40)
+    rope = A.Rope(64)
+    return {
+        "rope": lambda s: rope.apply(i32(3), q, k, stream=s),
+        "rope of strided rows": lambda s: rope.apply(i32(3), q[:, ::2], stream=s)[:1],
+        "read": lambda s: cache.read(0, batch, stream=s),
+        "attention": lambda s: (A.tree_attention(q, cache, 0, batch, stream=s),),
+        "logprobs": lambda s: L.token_logprobs(x, i32(3, 2), n_top=4, entropy=True, stream=s),
+    }
+
+
+@pytest.mark.parametrize("stream", [None, 0, 7])
+@pytest.mark.parametrize("name", list(calls()))
+def test_results_are_memory_of_the_calls_stream(monkeypatch, name, stream):
+    """The allocator gives a block to the work of one stream: results have to come from the stream that writes them, and
+    stay until the current stream is done with them."""
+    call = calls()[name]
+    dev = Streams(monkeypatch)
+    results = call(stream)
+    assert dev.launched == [stream]
+    where = dict(dev.made)
+    assert dev.made and all(s == (stream or 0) for s in where.values())
+    assert all(t.data_ptr() in where for t in results)
+    for t in results:
+        assert ((t.data_ptr(), 0) in dev.kept) == (stream == 7)

@@ -1,0 +1,77 @@
+"""Edges of the serving operators on the GPU: other streams, pools of other writers, bounds, captures, layouts."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from m3_avm_b200 import _lib
+from tests import serving_ref as R
+from tests.test_serving_gpu import assert_within, randn, roomy, status
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    status()
+    yield
+    assert status() == 0
+
+
+# ---------------------------------------------------------------- streams
+def stream_of(t):
+    """The stream whose memory t is, by the allocator."""
+    for seg in torch.cuda.memory_snapshot():
+        if seg["address"] <= t.data_ptr() < seg["address"] + seg["total_size"]:
+            return seg["stream"]
+    raise AssertionError("not the allocator's memory")
+
+
+def step_calls(seed=0):
+    """Every operator on the same inputs: name -> call(stream)."""
+    from m3_avm_b200.attention import KvCache, Rope, tree_attention
+    from m3_avm_b200.logprobs import token_logprobs
+
+    batch, pages, _, _ = R.make_batch([70, 9], [3, 2], 16)
+    cache = KvCache(8, 1, 2, 64, 16, pages)
+    full = R.whole(batch, [70, 9], [3, 2])
+    cache.write(0, randn(1, full.n_tokens, 2, 64), randn(2, full.n_tokens, 2, 64), full)
+    q, pos = randn(3, 5, 8, 64), torch.arange(5, dtype=torch.int32).cuda()
+    x, rope = randn(4, 5, 3000), Rope(64)
+    tokens = torch.zeros(5, 1, dtype=torch.int32).cuda()
+    ws = torch.empty(cache.attention_workspace(8, F32, 3), dtype=torch.uint8, device="cuda")
+    return {
+        "rope": lambda s: rope.apply(pos, q, q[:, :2], stream=s),
+        "read": lambda s: cache.read(0, full, stream=s),
+        "attention": lambda s: (tree_attention(q, cache, 0, batch, stream=s),),
+        "attention with a workspace": lambda s: (tree_attention(q, cache, 0, batch, workspace=ws, stream=s),),
+        "logprobs": lambda s: tuple(token_logprobs(x, tokens, n_top=20, entropy=True, stream=s)),
+    }
+
+
+@pytest.mark.parametrize("name", ["rope", "read", "attention", "attention with a workspace", "logprobs"])
+def test_calls_on_a_stream_of_their_own_beside_a_busy_current_one(name):
+    call = step_calls()[name]
+    want = call(None)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    big = torch.full((4096, 4096), 1.0, device="cuda")
+    for _ in range(5):
+        for _ in range(4):
+            (big @ big).sum()  # pending work on blocks that are free again
+        got = call(side.cuda_stream)
+        assert all(stream_of(t) == side.cuda_stream for t in got)
+        for t in got:
+            t.record_stream(side)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.current_stream().synchronize()
+    with torch.cuda.stream(side):  # the default stream by its handle
+        got = call(0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and stream_of(a) == 0 for a, b in zip(got, want))
