@@ -125,6 +125,29 @@ std::vector<DevState> g_dev;
 
 int g_ndev = -1;
 
+// The status words of the current device, zeroed.  The first call of a process
+// may be one that is being captured, on any stream: an allocation would end a
+// capture in its default mode, so the thread leaves that mode for it, and the
+// zeros are written on a stream of their own, which no capture waits for.
+int make_status(uint32_t** out) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  M3G_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+  void* p = nullptr;
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMalloc(&p, 256);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) {
+    cudaFree(p);
+    return cuda_fail(e, "status words");
+  }
+  *out = static_cast<uint32_t*>(p);
+  return M3G_OK;
+}
+
 int dev_state(int device, DevState** out) {
   std::lock_guard<std::mutex> lk(g_dev_mu);
   if (g_ndev <= 0) {
@@ -143,10 +166,7 @@ int dev_state(int device, DevState** out) {
     M3G_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
     M3G_CUDA(cudaDeviceGetAttribute(&d.smem_per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device));
     M3G_CUDA(cudaDeviceGetAttribute(&d.smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device));
-    void* p = nullptr;
-    M3G_CUDA(cudaMalloc(&p, 256));
-    M3G_CUDA(cudaMemset(p, 0, 256));
-    d.status = static_cast<uint32_t*>(p);
+    if (int rc = make_status(&d.status)) return rc;
     d.ready = true;
     M3G_CUDA(cudaSetDevice(prev));
   }

@@ -75,3 +75,38 @@ def test_calls_on_a_stream_of_their_own_beside_a_busy_current_one(name):
         got = call(0)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) and stream_of(a) == 0 for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------- captures
+CAPTURED = """
+import torch
+from m3_avm_b200.attention import KvBatch, KvCache, Rope, tree_attention
+from m3_avm_b200.logprobs import token_logprobs
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()
+cache = KvCache(8, 1, 2, 64, 16, 4)
+batch = KvBatch(i32(0, 3), i32(0), i32(2, 1).view(1, 2), 3, 3, 32)
+q, k, v, pos = torch.randn(3, 4, 64).cuda(), torch.randn(3, 2, 64).cuda(), torch.randn(3, 2, 64).cuda(), i32(0, 1, 2)
+head, rope = torch.randn(256, 500).cuda(), Rope(64)
+def step():
+    a, b = rope.apply(pos, q, k)
+    cache.write(0, b, v, batch)
+    o = tree_attention(a, cache, 0, batch)
+    kk, vv = cache.read(0, batch)
+    return [a, b, o, kk, vv] + [t for t in token_logprobs(o.view(3, 256), n_top=3, entropy=True) if t is not None]
+torch.mm(head.t()[:2], head)  # cuBLAS is not what is tested
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    done = subprocess.run([sys.executable, "-c", CAPTURED], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__))))
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
