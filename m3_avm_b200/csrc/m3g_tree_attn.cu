@@ -15,7 +15,7 @@
 // other one.  q is an exact f16 operand for F16 and BF16 (its rows are scaled by
 // a power of two); for F32 q and p * d are two f16 parts, hi + lo, 22 bits.
 // So that p * d stays in f16's normal range whatever V's scale, d is taken
-// relative to a power of two dref >= every d seen by the warp; when it grows,
+// relative to a power of two dref >= every |d| seen by the warp; when it grows,
 // the sums are rescaled (rare).
 //
 // Inside a CTA each of 4 warps owns every fourth group of 32 positions and a
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(
         grew = grew || mn > m[i];
         m[i] = mn;
       }
-      // V's scales: the largest of this step against dref
+      // V's scales: the largest magnitude of this step against dref (another writer's pool may hold scales below zero)
       uint32_t dv[NT][NB];
       __half2 big = __half2half2(__ushort_as_half(0));
 #pragma unroll
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(
           dv[nt][0] = x.x; dv[nt][1] = x.y;
         }
 #pragma unroll
-        for (int h = 0; h < NB; ++h) big = __hmax2(big, *reinterpret_cast<const __half2*>(&dv[nt][h]));
+        for (int h = 0; h < NB; ++h) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&dv[nt][h])));
       }
 #pragma unroll
       for (int x = 1; x < 4; x <<= 1) big = __hmax2(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));

@@ -19,7 +19,7 @@
 // activations, whose own step is as fine, K as two f16 parts (hi + lo, exact)
 // in two MMAs and the weights as two (with one, a result was off by 1.6 times what
 // rounding it to f16 costs, with two 1.35 times, for 12 % of the time); otherwise
-// weights as f16.  A group of 16 positions with a scale past 500 (a
+// weights as f16.  A group of 16 positions with a scale past +-500 (a
 // value could pass the f16 range) is taken at 2^-7, which its scores or weights
 // get back.
 //
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
           const int at16 = key * NB + (Q8 ? col >> 1 : col);
           d[j] = key < have ? sc[at16] : __ushort_as_half(0);
           const __half dv = is_v ? d[j] : key < have ? sc[16 * NB + at16] : __ushort_as_half(0);
-          plain = plain && d[j] <= lim && dv <= lim;  // NaN: not plain
+          plain = plain && __habs(d[j]) <= lim && __habs(dv) <= lim;  // NaN: not plain
         }
         int flags = 0;
         if (!__all_sync(0xFFFFFFFFu, plain)) {
@@ -584,8 +584,8 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
           for (int b = lane; b < 16 * NB; b += 32) {
             if (b / NB >= have) continue;
             const __half dv = sc[is_v ? b : 16 * NB + b];
-            odd_k |= !is_v && sc[b] > lim;
-            odd_v |= (dv > lim ? 1 : 0) | (__hisnan(dv) ? 2 : 0);
+            odd_k |= !is_v && __habs(sc[b]) > lim;
+            odd_v |= (__habs(dv) > lim ? 1 : 0) | (__hisnan(dv) ? 2 : 0);
           }
           flags = (__any_sync(0xFFFFFFFFu, odd_k) ? 1 : 0) | (__any_sync(0xFFFFFFFFu, odd_v & 1) ? 2 : 0) |
                   (__any_sync(0xFFFFFFFFu, odd_v & 2) && c >= first_tail ? 4 : 0);

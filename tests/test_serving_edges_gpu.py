@@ -110,3 +110,61 @@ def test_first_calls_of_a_process_can_be_captured():
     done = subprocess.run([sys.executable, "-c", CAPTURED], capture_output=True, text=True, timeout=300,
                           cwd=os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__))))
     assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+# ---------------------------------------------------------------- pools of other writers
+def planes(cache, layer=0):
+    """The layer's planes as the header lays them out: K codes, K scales, V codes, V scales."""
+    cb = cache.head_dim if cache.dtype == 8 else cache.head_dim // 2
+    nb = cache.head_dim // 32
+    rows = cache.n_pages * cache.n_kv_heads * cache.page_size
+    at, out = layer * rows * 2 * (cb + 2 * nb), []
+    for _ in range(2):
+        out.append(cache.pool[at:at + rows * cb].view(cache.n_pages, cache.n_kv_heads, cache.page_size, cb))
+        at += rows * cb
+        out.append(cache.pool[at:at + rows * 2 * nb].view(F16).view(cache.n_pages, cache.n_kv_heads, cache.page_size, nb))
+        at += rows * 2 * nb
+    return out
+
+
+def flip(cache, where):
+    """The blocks that `where` picks with the opposite sign of scale and codes: the same values."""
+    for codes, scales in (planes(cache)[:2], planes(cache)[2:]):
+        pick = where(scales.shape)
+        scales.copy_(torch.where(pick, -scales, scales))
+        wide = pick.repeat_interleave(codes.shape[-1] // scales.shape[-1], -1)
+        if cache.dtype == 8:
+            neg = (256 - codes.int()).to(torch.uint8)
+        else:
+            lo, hi = codes.int() & 15, codes.int() >> 4
+            neg = ((16 - lo) % 16 + 16 * ((16 - hi) % 16)).to(torch.uint8)
+        codes.copy_(torch.where(wide, neg, codes))
+
+
+@pytest.mark.parametrize("every", [True, False])
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,hd,large", [(F32, 64, False), (F16, 128, False), (BF16, 128, False), (BF16, 64, True),
+                                            (F16, 128, True)])
+def test_attention_scales_below_zero(dtype, hd, large, q8, every):
+    from m3_avm_b200.attention import KvCache, tree_attention
+
+    batch, pages, _, _ = R.make_batch([150], [4], 16)
+    heads = 64 if large else 4
+    for size in (1.0, 3e5 if q8 else 2e4):  # scales of up to 1e4, in f16's range
+        cache = KvCache(8 if q8 else 2, 1, 1, hd, 16, pages)
+        full = R.whole(batch, [150], [4])
+        k, v = randn(1, 154, 1, hd), randn(2, 154, 1, hd, scale=size)
+        cache.write(0, k, v, full)
+        g = torch.Generator().manual_seed(4)
+        flip(cache, lambda s: torch.ones(s, dtype=torch.bool).cuda() if every else
+             (torch.rand(s, generator=g) < 0.5).cuda())
+        kd, vd = (x.double().cpu() for x in cache.read(0, full))
+        assert torch.equal(kd.float(), R.quantised(k, q8)) and torch.equal(vd.float(), R.quantised(v, q8))
+        q = randn(3, 4, heads, hd, dtype=dtype)
+        got = tree_attention(q, cache, 0, roomy(batch, 16) if large else batch)
+        bits = [np.tril(np.ones((4, 4), bool))]
+        want, vmax, smag = R.attention(q, [kd], [vd], [150], [4], bits, hd ** -0.5)
+        bound = R.attention_bound(want, vmax, smag, dtype)
+        past = want.abs() + bound >= torch.finfo(dtype).max  # F16: the nearest value may be infinite
+        got = torch.where(past & torch.isinf(got.cpu()) & (torch.sign(got.cpu()) == torch.sign(want)), want, got.double().cpu())
+        assert_within(got, want, bound)
