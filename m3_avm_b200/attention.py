@@ -265,6 +265,8 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     of word i / 32 says whether the token sees new token i of its sequence; None: all up to and including itself.
     `workspace`: a uint8 tensor of cache.attention_workspace(heads, q.dtype, batch.max_tokens) bytes, used by one call
     at a time (allocated here when None)."""
+    if scale is not None and not ctypes.c_float(scale).value > 0:  # in 32 bits, where 0 stands for the default
+        _fail("scale must be positive")
     device, dtype = _device(q), act_dtype(q)
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
     heads = shape[1]
@@ -281,8 +283,6 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
         words = mask.shape[-1] if mask.dim() == 2 else 0
         _check_ints("mask", mask, device, (batch.n_tokens, words))
         bits = mask.data_ptr()
-    if scale is not None and not scale > 0:
-        _fail("scale must be positive")
     if workspace is None:
         workspace = _on(device, stream, cache.pool.new_empty,
                         cache.attention_workspace(heads, q.dtype, batch.max_tokens))

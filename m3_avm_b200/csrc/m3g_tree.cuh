@@ -40,6 +40,11 @@ __device__ __forceinline__ float tex2(float x) {
   return y;
 }
 
+// The factor that turns raw scores into base-2 exponents.  Never 0: -inf, the score
+// of what a row does not see, times 0 is NaN.  (Raw scores stay below 2^42, so
+// that with factors up to this one all seen scores are 0 to 2^-84.)
+__device__ __forceinline__ float score_factor(float f) { return fmaxf(f, 0x1p-126f); }
+
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

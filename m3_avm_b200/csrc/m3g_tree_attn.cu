@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(
       // times a power of two that puts the largest into [2^10, 2^11)
       const int e = max(60, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
       const float up = __uint_as_float(static_cast<uint32_t>(264 - e) << 23);
-      row_scale[i] = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 10) << 23);
+      row_scale[i] = score_factor(a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 10) << 23));
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll

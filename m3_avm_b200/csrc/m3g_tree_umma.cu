@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
         }
         const int e = max(60, min(254, static_cast<int>(__float_as_uint(most) >> 23)));
         const float up = __uint_as_float(static_cast<uint32_t>(258 - e) << 23);
-        cs = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 4) << 23);
+        cs = score_factor(a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(e - 4) << 23));
 #pragma unroll 1
         for (int i0 = 0; i0 < HD / 8; i0 += PART) {
 #pragma unroll

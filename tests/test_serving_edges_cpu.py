@@ -6,6 +6,7 @@ import torch
 
 from m3_avm_b200 import attention as A
 from m3_avm_b200 import logprobs as L
+from m3_avm_b200._lib import M3GError
 
 
 def i32(*s):
@@ -77,3 +78,13 @@ def test_results_are_memory_of_the_calls_stream(monkeypatch, name, stream):
     assert all(t.data_ptr() in where for t in results)
     for t in results:
         assert ((t.data_ptr(), 0) in dev.kept) == (stream == 7)
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), 1e-50])
+def test_scales_that_are_not_positive_in_32_bits(scale):
+    """1e-50 is 0 in 32 bits, which the library takes for 1 / sqrt(head_dim)."""
+    cache = A.KvCache(8, 1, 2, 64, 16, 4, pool=torch.zeros(4 * 2 * 16 * 2 * 68, dtype=torch.uint8))
+    batch = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64)
+    with pytest.raises(M3GError, match="scale must be positive"):
+        A.tree_attention(torch.zeros(3, 4, 64), cache, 0, batch, scale=scale)

@@ -168,3 +168,23 @@ def test_attention_scales_below_zero(dtype, hd, large, q8, every):
         past = want.abs() + bound >= torch.finfo(dtype).max  # F16: the nearest value may be infinite
         got = torch.where(past & torch.isinf(got.cpu()) & (torch.sign(got.cpu()) == torch.sign(want)), want, got.double().cpu())
         assert_within(got, want, bound)
+
+
+# ---------------------------------------------------------------- scores and bounds
+@pytest.mark.parametrize("dtype,large", [(F32, False), (BF16, False), (F16, True), (BF16, True)])
+@pytest.mark.parametrize("scale,qscale", [(1e-24, 0.0), (1e-44, 1.0), (1e-30, 1e-20)])
+def test_attention_scores_that_underflow(dtype, large, scale, qscale):
+    """Scores of (nearly) nothing: the mean of what each row sees."""
+    from m3_avm_b200.attention import KvCache, tree_attention
+
+    batch, pages, _, _ = R.make_batch([40], [5], 16)
+    cache = KvCache(8, 1, 1, 64, 16, pages)
+    full = R.whole(batch, [40], [5])
+    k, v = randn(1, 45, 1, 64), randn(2, 45, 1, 64)
+    cache.write(0, k, v, full)
+    q = randn(3, 5, 64 if large else 4, 64, scale=qscale, dtype=dtype)
+    got = tree_attention(q, cache, 0, roomy(batch, 16) if large else batch, scale=scale)
+    bits = [np.tril(np.ones((5, 5), bool))]
+    want, vmax, smag = R.attention(q, [R.quantised(k, True).double()], [R.quantised(v, True).double()], [40], [5], bits,
+                                   scale)
+    assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
