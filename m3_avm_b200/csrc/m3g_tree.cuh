@@ -56,8 +56,11 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t x) {
 // Low n bits set, n clamped to 0 .. 32.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
-// A sequence's work in chunks of CHUNK positions and tiles of TILE rows.  (All
-// chunks of a batch number less than 2^31: the host's check.)
+// A sequence's work in chunks of CHUNK positions and tiles of TILE rows.
+// kTreeMost: chunks that a batch may come to.  The host refuses what its tokens and
+// bounds could exceed; tree_share looks at what the arrays really say (sequences
+// that overlap can come to more), so that every sum of chunks fits an int.
+constexpr long long kTreeMost = (1ll << 31) - 1024;
 template <int CHUNK, int TILE>
 struct SeqWork {
   SeqView v;
@@ -67,6 +70,7 @@ struct SeqWork {
     tiles = (v.n * a.group + TILE - 1) / TILE;
   }
   __device__ __forceinline__ int total(int kvh) const { return chunks * tiles * kvh; }
+  __device__ __forceinline__ long long total64(int kvh) const { return static_cast<long long>(chunks) * tiles * kvh; }
 };
 
 // A CTA's share of all chunks and where it starts: G CTAs have work, the first
@@ -79,7 +83,7 @@ struct TreeShare {
 };
 
 struct ShareScratch {
-  int red[32], found[2];
+  int red[32], red2[32], found[2];
 };
 
 // All threads of the CTA (THREADS, whole warps); false: nothing to do.  LEAST:
@@ -91,18 +95,27 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, ShareScratch& sc, 
   const int n_seqs = static_cast<int>(a.b.n_seqs), kvh = a.p.kvh;
   using Work = SeqWork<CHUNK, TILE>;
   bool bad = false;
-  int mine = 0, own0 = 0;
+  long long mine = 0, own0 = 0;
 #pragma unroll 1
   for (int s = tid; s < n_seqs; s += THREADS) {
-    const int own = Work(a, s, &bad).total(kvh);
+    const long long own = min(Work(a, s, &bad).total64(kvh), kTreeMost + 1);
     if (s == tid) own0 = own;
     mine += own;
   }
-  if (bad && blockIdx.x == 0) atomicOr(a.p.status, kStatusBadBatch);
-  mine = __reduce_add_sync(0xFFFFFFFFu, mine);
-  if (lane == 0) sc.red[warp] = mine;
+  mine = min(mine, kTreeMost + 1);  // added up in two parts, of 24 bits and of the others
+  const int lo = __reduce_add_sync(0xFFFFFFFFu, static_cast<int>(mine & 0xFFFFFF));
+  const int hi = __reduce_add_sync(0xFFFFFFFFu, static_cast<int>(mine >> 24));
+  if (lane == 0) {
+    sc.red[warp] = lo;
+    sc.red2[warp] = hi;
+  }
   __syncthreads();
-  const int W = __reduce_add_sync(0xFFFFFFFFu, lane < WARPS ? sc.red[lane] : 0);
+  const int part = lane < WARPS ? sc.red[lane] : 0, above = lane < WARPS ? sc.red2[lane] : 0;
+  const long long all = __reduce_add_sync(0xFFFFFFFFu, part & 0xFFFFFF) +
+                        (static_cast<long long>(__reduce_add_sync(0xFFFFFFFFu, above + (part >> 24))) << 24);
+  if (all > kTreeMost) bad = true;  // the batch as a whole: nothing is done
+  if (bad && blockIdx.x == 0) atomicOr(a.p.status, kStatusBadBatch);
+  const int W = all > kTreeMost ? 0 : static_cast<int>(all);
   const int b = blockIdx.x, G = min(static_cast<int>(gridDim.x), (W + LEAST - 1) / LEAST);
   if (tid == 0) a.desc[b].x = -1;
   if (b >= G) return false;
@@ -114,7 +127,7 @@ __device__ __forceinline__ bool tree_share(const TreeArgs& a, ShareScratch& sc, 
   int before = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < n_seqs; s0 += THREADS) {
-    int own = own0;
+    int own = static_cast<int>(own0);
     if (s0) own = s0 + tid < n_seqs ? Work(a, s0 + tid, &bad).total(kvh) : 0;
     int up = own;  // inclusive scan
 #pragma unroll
@@ -238,7 +251,7 @@ cudaError_t launch_join(const TreeArgs& a, int grid, cudaStream_t st) {
 
 // The form on the fifth-generation tensor cores (m3g_tree_umma.cu): 16-bit
 // types, units of 128 rows.
-constexpr int kUmmaTile = 128;
+constexpr int kUmmaTile = 128, kUmmaChunk = 64;  // rows, positions
 cudaError_t launch_tree_umma(const TreeArgs& a, uint32_t dtype, bool q8, int sms, cudaStream_t st);
 
 }  // namespace m3g

@@ -616,6 +616,20 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
     return host_fail(M3G_EINVAL, "workspace of %llu bytes (16-byte aligned, %llu needed)",
                      static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(need));
+  a.cap = seq_cap(*b, l->page_size);
+  a.n_heads = static_cast<int>(n_heads);
+  a.group = static_cast<int>(n_heads / l->n_kv_heads);
+  const uint64_t most_rows = static_cast<uint64_t>(b->max_tokens) * a.group;  // of a sequence's KV head
+  const uint64_t tiles = (most_rows + kUmmaTile - 1) / kUmmaTile;
+  const bool umma = can_use_umma(l, dtype, n_heads, b->max_tokens) &&
+                    b->n_seqs * l->n_kv_heads * tiles * ((static_cast<uint64_t>(a.cap) + 63) / 64) >= kUmmaChunks;
+  // Chunks that the batch can come to in this form: no sequence has more than
+  // max_tokens, all together no more than n_tokens.
+  const uint64_t tile = umma ? kUmmaTile : kTile, chunk = umma ? kUmmaChunk : kChunk;
+  const uint64_t units = l->n_kv_heads * std::min(b->n_seqs * ((most_rows + tile - 1) / tile),
+                                                  static_cast<uint64_t>(b->n_tokens) * a.group / tile + b->n_seqs);
+  if (most_rows >= (1ull << 31) || units * ((static_cast<uint64_t>(a.cap) + chunk - 1) / chunk) > kTreeMost)
+    return host_fail(M3G_EINVAL, "batch too large (sequences x heads x tokens x length)");
   int dev = 0, sms = 0;
   if (int rc = serve_device(&dev, &a.p.status)) return rc;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -629,17 +643,6 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   a.out = *out;
   a.mask = mask;
   a.mask_words = static_cast<int>(mask_words);
-  a.cap = seq_cap(*b, l->page_size);
-  a.n_heads = static_cast<int>(n_heads);
-  a.group = static_cast<int>(n_heads / l->n_kv_heads);
-  // chunks of 64 positions at worst, in tiles of 16 rows
-  const uint64_t units = static_cast<uint64_t>(b->n_seqs) * l->n_kv_heads *
-                         ((static_cast<uint64_t>(b->max_tokens) * a.group + kTile - 1) / kTile);
-  if (static_cast<uint64_t>(b->max_tokens) * a.group >= (1ull << 31) || units >= (1ull << 31) || units * (static_cast<uint64_t>(a.cap) / 64 + 1) >= (1ull << 31))
-    return host_fail(M3G_EINVAL, "batch too large (sequences x heads x tokens x length)");
-  const uint64_t tiles = (static_cast<uint64_t>(b->max_tokens) * a.group + kUmmaTile - 1) / kUmmaTile;
-  const bool umma = can_use_umma(l, dtype, n_heads, b->max_tokens) &&
-                    b->n_seqs * l->n_kv_heads * tiles * ((static_cast<uint64_t>(a.cap) + 63) / 64) >= kUmmaChunks;
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(a.p.hd));
   const cudaStream_t st = serve_stream(stream);
   const bool q8 = l->dtype == M3G_DTYPE_Q8_0;

@@ -49,7 +49,7 @@
 namespace m3g {
 namespace {
 
-constexpr int kUChunk = 64;
+constexpr int kUChunk = kUmmaChunk;
 constexpr int kUThreads = 512;                       // softmax, K, V and issuing warpgroups
 constexpr int kUCols = 256;                          // TMEM columns of a CTA
 constexpr int kOCol = 2 * kUChunk;                   // O behind the two score buffers

@@ -88,3 +88,32 @@ def test_scales_that_are_not_positive_in_32_bits(scale):
     batch = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64)
     with pytest.raises(M3GError, match="scale must be positive"):
         A.tree_attention(torch.zeros(3, 4, 64), cache, 0, batch, scale=scale)
+
+
+def test_attention_bounds_that_are_and_are_not_too_large():
+    """Bounds count as what the batch's tokens could come to, not as if every sequence had the most of all."""
+    import ctypes
+
+    from m3_avm_b200 import _lib
+    from tests.conftest import HAS_CUDA
+
+    if HAS_CUDA:
+        pytest.skip("host pointers: only where nothing can be launched")
+    buf = (ctypes.c_uint8 * (1 << 16))()
+    p = ctypes.addressof(buf) // 64 * 64 + 64
+
+    def call(n_seqs, n_tokens, max_tokens, max_len, dtype):
+        lay = _lib.KvLayout(8, 1, 8, 128, 64, 1000)
+        bat = _lib.KvBatchArgs(p, p, p, n_seqs, 1 << 14, n_tokens, max_tokens, max_len)
+        a, b = _lib.Rows(p, 4096, 128), _lib.Rows(p + 8192, 4096, 128)
+        return _lib.load().m3g_tree_attn_dev(ctypes.byref(lay), p, 0, ctypes.byref(bat), dtype, ctypes.byref(a), 32,
+                                             None, 0, 0.0, ctypes.byref(b), p, 1 << 40, None)
+
+    for dtype in (0, 1, 30):
+        # one prompt chunk beside single tokens
+        assert call(256, 2303, 2048, 131072, dtype) == _lib.M3G_ECUDA
+        assert call(1000, 1999, 1000, 1 << 20, dtype) == _lib.M3G_ECUDA
+        # 2^31 chunks and more
+        assert call(1 << 20, 1 << 20, 1, 1 << 20, dtype) == _lib.M3G_EINVAL
+        assert call(4096, 1 << 24, 1 << 12, 1 << 20, dtype) == _lib.M3G_EINVAL
+        assert call(1, 1 << 30, 1 << 30, 64, dtype) == _lib.M3G_EINVAL

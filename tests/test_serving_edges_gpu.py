@@ -188,3 +188,42 @@ def test_attention_scores_that_underflow(dtype, large, scale, qscale):
     want, vmax, smag = R.attention(q, [R.quantised(k, True).double()], [R.quantised(v, True).double()], [40], [5], bits,
                                    scale)
     assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
+
+
+def test_batch_of_large_bounds():
+    """Bounds that only one sequence could reach refuse no batch whose tokens are few."""
+    from m3_avm_b200.attention import KvBatch, KvCache, tree_attention
+
+    n = 300
+    ctx, new = [5 + i % 40 for i in range(n)], [1] * n
+    new[7] = 30
+    batch, pages, table, _ = R.make_batch(ctx, new, 64)
+    wide = torch.full((n, 2048), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    cache = KvCache(8, 1, 8, 64, 64, pages)
+    full = R.whole(batch, ctx, new)
+    cache.write(0, randn(1, full.n_tokens, 8, 64), randn(2, full.n_tokens, 8, 64), full)
+    for dtype in (BF16, F32):
+        q = randn(3, sum(new), 32, 64, dtype=dtype)
+        tight = tree_attention(q, cache, 0, batch)
+        got = tree_attention(q, cache, 0, KvBatch(batch.q_start, batch.ctx_len, wide.cuda(), sum(new), 2048, 131072))
+        assert float((got.float() - tight.float()).abs().max()) < 0.02
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sequences_that_overlap_past_all_bounds_are_refused_whole(dtype):
+    """2^12 starts that go back and forth, so that every second sequence claims the same 2^10 tokens, behind 2^20
+    positions each: 2^33 chunks and more, where the bounds allow 2^29."""
+    from m3_avm_b200.attention import KvBatch, KvCache, tree_attention
+
+    n, t = 1 << 12, 1 << 10
+    starts = torch.zeros(n + 1, dtype=torch.int32)
+    starts[1::2] = t
+    cache = KvCache(8, 1, 8, 64, 1024, 1)
+    table = torch.zeros(n, 1024, dtype=torch.int32).cuda()
+    batch = KvBatch(starts.cuda(), torch.full((n,), 2 ** 20 - t, dtype=torch.int32).cuda(), table, t, t, 2 ** 20)
+    q = randn(1, t, 32, 64, dtype=dtype)
+    out = torch.full_like(q, 5.0)
+    tree_attention(q, cache, 0, batch, out=out)
+    assert status() == 16
+    assert bool((out == 5).all())
