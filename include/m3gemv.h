@@ -481,7 +481,9 @@ M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint3
  * f32.  Products take the cached codes exactly and p as f16 (F32: q and p in
  * two f16 parts); large BF16 calls with more than 48 rows (tokens times query
  * heads per KV head) take the cached values rounded to f16, F16 ones V's (and
- * p in two parts).
+ * p in two parts).  That form hands tiles between warps, whose waits are bounded
+ * ("attn_wait_us"): should one run out, the rows it was for become NaN and bit 0 of
+ * the device status word is set.
  * `workspace`: m3g_tree_attn_workspace() bytes (with the call's dtype, n_heads
  * and max_tokens) of device memory, 16-byte aligned, contents free, used by
  * one call at a time. */
@@ -521,7 +523,9 @@ M3G_API uint64_t m3g_launch_count(void);
  * "max_stages"), "force_generic" (route every GEMV through the
  * row-straddling generic kernel) and "peer_wait_us" (limit, in microseconds,
  * of a kernel's wait for a counter bumped by another GPU or producer; default
- * 2000000; read when a GEMV is enqueued or a decode step captured), "tc8"
+ * 2000000; read when a GEMV is enqueued or a decode step captured), "attn_wait_us"
+ * (limit of a wait inside m3g_tree_attn_dev's form of 128-row tiles; default
+ * 2000000, 0 lets no wait last; read when a call is enqueued), "tc8"
  * (1: batch-1 Q4_K GEMVs with in_dim <= 4096 on the tcgen05 kind::i8 kernel;
  * default 0, the mma.sync kernel being faster), "shard_p2p" (see
  * m3g_shard_create) and "offload_mapped" (1, default: host-buffer offload

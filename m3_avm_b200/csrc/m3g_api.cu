@@ -99,6 +99,7 @@ struct Tuning {
   int64_t umma_chains = 8;        // independent accumulators per super-block (capped by TMEM)
   int64_t offload_graph = 1;      // host-buffer offload calls replay one CUDA graph (copy in, GEMV, copy out)
   int64_t peer_wait_us = 2000000; // limit of a kernel's wait for a counter bumped by other GPUs
+  int64_t attn_wait_us = 2000000; // limit of a wait inside attention's 128-row form
   int64_t mma_tail_first = 1;     // tensor-core GEMV: a CTA's partial row group first
   int64_t offload_mapped = 1;     // batch-1 host-buffer calls: x, y, status through mapped pinned memory
   int64_t shard_p2p = -1;         // shard contexts: 1 rows exchanged by peer stores from the GEMV epilogue, 0 NCCL,
@@ -724,6 +725,7 @@ bool fused_plannable(int device, uint32_t dtype, long long in_dim, long long row
   return plan_mma(f, in_dim, rows, w16, kAligned, *ds, mp, false);
 }
 unsigned long long peer_wait_ns() { return static_cast<unsigned long long>(g_tune.peer_wait_us) * 1000ull; }
+uint64_t attn_wait_us() { return static_cast<uint64_t>(g_tune.attn_wait_us); }
 bool decode_shard_ffn_enabled() { return g_tune.decode_shard_ffn != 0; }
 
 void count_launches(int n) { g_launches.fetch_add(static_cast<uint64_t>(n), std::memory_order_relaxed); }
@@ -781,6 +783,7 @@ int m3g_set_tuning(const char* key, int64_t value) {
   else if (!strcmp(key, "umma")) g_tune.umma = value != 0;
   else if (!strcmp(key, "offload_graph")) g_tune.offload_graph = value != 0;
   else if (!strcmp(key, "umma_chains") && value >= 1 && value <= 8) g_tune.umma_chains = value;
+  else if (!strcmp(key, "attn_wait_us") && value >= 0 && value <= 60000000) g_tune.attn_wait_us = value;
   else if (!strcmp(key, "peer_wait_us") && value >= 1 && value <= 60000000) g_tune.peer_wait_us = value;
   else if (!strcmp(key, "mma_tail_first")) g_tune.mma_tail_first = value != 0;
   else if (!strcmp(key, "offload_mapped")) g_tune.offload_mapped = value != 0;

@@ -227,6 +227,8 @@ bool plan_tc8(long long in_dim, long long rows, const uint8_t* w, const float* x
               Tc8Plan& p);
 cudaError_t launch_tc8(const Tc8Plan& p, const uint8_t* w, cudaStream_t st, bool pdl);
 
+// Limit of a wait inside attention's 128-row form ("attn_wait_us").
+uint64_t attn_wait_us();
 // Adds to the count of enqueued kernels (m3g_launch_count).
 void count_launches(int n);
 

@@ -27,6 +27,7 @@ struct TreeArgs {
   int mask_words, n_heads, group;
   int vec, vec_out;  // q, result rows are 16-byte aligned
   float scale;
+  uint32_t wait_polls, wait_ns;  // of the 128-row form's waits: polls, and the longest that each takes
 };
 
 template <int HD, int TILE>

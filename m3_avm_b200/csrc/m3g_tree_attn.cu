@@ -644,6 +644,9 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* l, const void* pool, uint32_t
   a.mask = mask;
   a.mask_words = static_cast<int>(mask_words);
   a.scale = scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(a.p.hd));
+  const uint64_t wait_us = attn_wait_us();
+  a.wait_ns = static_cast<uint32_t>(std::min<uint64_t>(2000, 1000 * wait_us));
+  a.wait_polls = static_cast<uint32_t>(std::max<uint64_t>(1, wait_us / 2));
   const cudaStream_t st = serve_stream(stream);
   const bool q8 = l->dtype == M3G_DTYPE_Q8_0;
   const cudaError_t e = umma ? launch_tree_umma(a, dtype, q8, sms, st)

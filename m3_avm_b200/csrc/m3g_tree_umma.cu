@@ -39,8 +39,14 @@
 // clock64 trace showed 5100 cycles a chunk with one issuing thread for both
 // products, 4700 with the issuing done by the unpacking warps.  Registers go
 // from the other groups to the softmax.  256 TMEM columns: two score buffers
-// (weights written over them) and O.  Every wait is bounded; a timeout raises
-// the copy-timeout bit and the CTA runs to its end without waiting again.
+// (weights written over them) and O.
+//
+// Every wait is bounded (wait_polls polls of wait_ns at most).  A role whose wait
+// gives up raises the copy-timeout bit and the CTA's abort word, which ends the
+// others' waits, and neither issues nor arrives any more: a phase that a barrier
+// completes is always one whose work was done.  At the end of the piece the issuing
+// warps wait (bounded too) for their products and copies in flight; the rows of
+// this piece and of the CTA's later ones become NaN.
 #include <type_traits>
 
 #include "m3g_tcgen05.cuh"
@@ -53,7 +59,7 @@ constexpr int kUChunk = kUmmaChunk;
 constexpr int kUThreads = 512;                       // softmax, K, V and issuing warpgroups
 constexpr int kUCols = 256;                          // TMEM columns of a CTA
 constexpr int kOCol = 2 * kUChunk;                   // O behind the two score buffers
-constexpr uint32_t kUPolls = 1u << 24;               // of a wait, after which it gives up
+constexpr uint32_t kSettlePolls = 1u << 20, kSettleNs = 2000;  // for work in flight when a wait gave up
 // log2 of the factor that all weights carry, and of the growth of a row's maximum
 // that is let pass: weights stay below 2^15.  Where V's groups at 2^-7 get their
 // factor back in the weights, less growth passes.  (A rescaling costs its warp
@@ -263,23 +269,23 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = uniform(tslot);
-  // Bounded by polls (each holds the thread for a while), and short: with 16 warps
-  // in four roles the kernel's loops have to stay within the instruction caches
-  // (with everything unrolled and inlined waits for instructions were the
-  // largest stall).
-  auto wait_one = [&](uint64_t* b, uint32_t parity) {  // by one lane
+  // Short: with 16 warps in four roles the kernel's loops have to stay within the
+  // instruction caches (with everything unrolled and inlined waits for instructions
+  // were the largest stall).
+  auto wait_one = [&](uint64_t* b, uint32_t parity) -> bool {  // by one lane; false: gave up
     uint32_t polls = 0;
-    while (!mbar_try_wait(b, parity)) {
-      if (++polls < kUPolls && !*abort_flag) continue;
+    while (!mbar_try_wait_for(b, parity, a.wait_ns)) {
+      if (++polls < a.wait_polls && !*abort_flag) continue;
       if (!*abort_flag) atomicOr(a.p.status, kStatusCopyTimeout);
       *abort_flag = 1;
-      break;
+      return false;
     }
+    return true;
   };
-  auto wait = [&](uint64_t* b, uint32_t parity) {  // by a warp
-    wait_one(b, parity);
-    __syncwarp();
+  auto wait = [&](uint64_t* b, uint32_t parity) -> bool {  // by a warp, the same for all lanes
+    return __all_sync(0xFFFFFFFFu, wait_one(b, parity));
   };
+  auto aborted = [&]() -> bool { return __any_sync(0xFFFFFFFFu, *abort_flag); };
   // The first thread of the V group finds the CTA's pieces.
   int at_seq = share.seq, at = share.first, before = share.before;
   auto next_piece = [&] {
@@ -320,8 +326,9 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
       const int row = pc.tile * kUmmaTile + tid;
       const bool live = row < pc.rows;
       const int token = live ? row / a.group : 0, hq = pc.head * a.group + row % a.group;
-      float cs;  // factor of the raw scores, in base 2
-      {
+      bool dead = aborted();  // the rows of this piece become NaN
+      float cs = 0.f;         // factor of the raw scores, in base 2
+      if (!dead) {
         // This thread's row, read for its largest value and read again, times a power of two that puts its largest into
         // [2^4, 2^5): room for K's f16 range in the f32 sums.
         const T* q = static_cast<const T*>(a.q.p) + (pc.q0 + token) * a.q.token_stride + hq * a.q.head_stride;
@@ -377,7 +384,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
       float m = -INFINITY, l = 0.f;
       uint32_t nan_blocks = 0u;
 #pragma unroll 1
-      for (int c = 0; c < n; ++c) {
+      for (int c = 0; c < n && !dead; ++c) {
         const uint32_t ph = it + c;
         const int buf = ph & 1, p0 = (pc.c0 + c) * kUChunk;
         const bool tail = p0 + kUChunk > pc.ctx;
@@ -386,19 +393,23 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
           vis[0] = tree_sees(a, pc.q0, token, pc.ctx, pc.len, p0);
           vis[1] = tree_sees(a, pc.q0, token, pc.ctx, pc.len, p0 + 32);
         }
-        wait(&bar.s_full[buf], (ph >> 1) & 1);
+        if (!wait(&bar.s_full[buf], (ph >> 1) & 1)) {
+          dead = true;
+          break;
+        }
         tc_fence_after();
         const int4 od = *reinterpret_cast<const int4*>(odd[ph & 3]);
         const int flags[4] = {od.x, od.y, od.z, od.w};
         const float lag = (od.x | od.y | od.z | od.w) & 2 ? kLagOddV : kLag;
-        auto rescale = [&](float mx, bool grows) {  // some row of the warp refers to a larger maximum from now on
+        // Some row of the warp refers to a larger maximum from now on; false: a wait gave up.
+        auto rescale = [&](float mx, bool grows) -> bool {
           const float f = grows ? tex2(m - mx) : 1.f;
           if (grows) {
             m = mx;
             l *= f;
           }
           if (c > 0) {
-            wait(&bar.s_free[buf ^ 1], ((ph - 1) >> 1) & 1);  // the results so far are there
+            if (!wait(&bar.s_free[buf ^ 1], ((ph - 1) >> 1) & 1)) return false;  // the results so far are there
             tc_fence_after();
 #pragma unroll 1
             for (int h = 0; h < HD / 16; ++h) {
@@ -409,6 +420,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
               tc_st16(tl + kOCol + 16 * h, x);
             }
           }
+          return true;
         };
         // The scores of a group of 16 positions, read while the one before is worked on.
         uint32_t x[2][16];
@@ -435,7 +447,10 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
             mx = fmaxf(mx, top * (flags[h] & 1 ? 128.f * cs : cs));
           }
           const bool grows = mx > m + lag || (m == -INFINITY && mx > -INFINITY);
-          if (__any_sync(0xFFFFFFFFu, grows)) rescale(mx, grows);
+          if (__any_sync(0xFFFFFFFFu, grows) && !rescale(mx, grows)) {
+            dead = true;
+            break;
+          }
           const float ref = m == -INFINITY ? 0.f : m - kLift;
           tc_ld16_start(tl + buf * kUChunk, x[0]);
 #pragma unroll
@@ -489,8 +504,12 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
             }
             const bool grows = mx > m + lag || (m == -INFINITY && mx > -INFINITY);
             if (!__any_sync(0xFFFFFFFFu, grows)) break;
-            rescale(mx, grows);
+            if (!rescale(mx, grows)) {
+              dead = true;
+              break;
+            }
           }
+          if (dead) break;
           tc_st16(tl + buf * kUChunk, *reinterpret_cast<uint32_t(*)[16]>(&p[0]));
           tc_st16(tl + buf * kUChunk + 16, *reinterpret_cast<uint32_t(*)[16]>(&p[16]));
         }
@@ -505,8 +524,12 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_ready[buf]);
       }
-      wait(&bar.s_free[(it + n - 1) & 1], ((it + n - 1) >> 1) & 1);
+      if (!dead) dead = !wait(&bar.s_free[(it + n - 1) & 1], ((it + n - 1) >> 1) & 1);
       tc_fence_after();
+      if (dead) {  // a NaN sum makes what is joined from this piece NaN too
+        m = 0.f;
+        l = NAN;
+      }
       {
         const bool whole = pc.whole;
         float* part = a.parts + static_cast<long long>(2 * blockIdx.x + (pc.c0 == 0)) * Part<HD, kUmmaTile>::kFloats;
@@ -515,7 +538,12 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
 #pragma unroll 1
         for (int h = 0; h < HD / 16; ++h) {
           uint32_t x[16];
-          tc_ld16(tl + kOCol + 16 * h, x);
+          if (dead) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = 0x7FC00000u;
+          } else {
+            tc_ld16(tl + kOCol + 16 * h, x);
+          }
           if (live) {
 #pragma unroll
             for (int q = 0; q < 16; q += 8) {
@@ -557,11 +585,12 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
       const int n = uniform(pc.n);
       if (!n) break;
       const int first_tail = (pc.ctx / kUChunk) - pc.c0;  // the first chunk with new tokens
+      const int todo = aborted() ? 0 : n;
 #pragma unroll 1
-      for (int c = 0; c < n; ++c) {
+      for (int c = 0; c < todo; ++c) {
         const uint32_t ph = it + c, rs = ph % NST;
         const uint8_t* st = raw + rs * raw_stage;
-        wait(&bar.raw[is_v][rs], (ph / NST) & 1);
+        if (!wait(&bar.raw[is_v][rs], (ph / NST) & 1)) break;
         const int have = held[is_v][rs][gw];
         // scales of this lane's pieces, and (K's warps) of its share of the group's V blocks
         __half d[PPL];
@@ -591,7 +620,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
                   (__any_sync(0xFFFFFFFFu, odd_v & 2) && c >= first_tail ? 4 : 0);
         }
         // K's tile is free once the last chunk's scores are done, V's once its results are.
-        if (c > 0) wait(is_v ? &bar.pv_done : &bar.k_free, (ph - 1) & 1);
+        if (c > 0 && !wait(is_v ? &bar.pv_done : &bar.k_free, (ph - 1) & 1)) break;
         if (!is_v && lane == 0) odd[ph & 3][gw] = flags;
         if (flags & (is_v ? 2 : 1)) {
 #pragma unroll
@@ -638,18 +667,20 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
       __syncthreads();
       const int n = uniform(pc.n);
       if (!n) break;
+      const int todo = aborted() ? 0 : n;
+      int c = 0;  // chunks that this lane has issued
       if (gw == 0) {
-        if (elect()) {
+        if (todo && elect()) {
         // S = Q K^T, into the buffer whose weights are used
         // (a descriptor's low 14 bits are the address in 16-byte units: steps are added to it)
         const uint64_t q0 = smem_desc(smem_addr(smem), G::kQStride, 128);
         const uint64_t k0 = smem_desc(smem_addr(smem + G::off_k), G::kStride, 128);
-        wait_one(&bar.q_ready, pn & 1);
+        const bool ready = wait_one(&bar.q_ready, pn & 1);
 #pragma unroll 1
-        for (int c = 0; c < n; ++c) {
+        for (; ready && c < todo; ++c) {
           const uint32_t ph = it + c, buf = ph & 1;
-          wait_one(&bar.k_ready, ph & 1);
-          if (c >= 2) wait_one(&bar.s_free[buf], ((ph >> 1) - 1) & 1);
+          if (!wait_one(&bar.k_ready, ph & 1)) break;
+          if (c >= 2 && !wait_one(&bar.s_free[buf], ((ph >> 1) - 1) & 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
@@ -662,14 +693,14 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
         }
         }
       } else if (gw == 1) {
-        if (elect()) {
+        if (todo && elect()) {
         // O += P V
         const uint64_t v0 = smem_desc(smem_addr(smem + G::off_v), 128, G::kStride);
 #pragma unroll 1
-        for (int c = 0; c < n; ++c) {
+        for (; c < todo; ++c) {
           const uint32_t ph = it + c, buf = ph & 1;
-          wait_one(&bar.v_ready, ph & 1);
-          wait_one(&bar.p_ready[buf], (ph >> 1) & 1);
+          if (!wait_one(&bar.v_ready, ph & 1)) break;
+          if (!wait_one(&bar.p_ready[buf], (ph >> 1) & 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kUChunk / 16; ++k)
@@ -692,10 +723,11 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
         };
         int page = page_of(0);
 #pragma unroll 1
-        for (int c = 0; c < n; ++c) {
+        for (; c < todo; ++c) {
           const uint32_t ph = it + c, rs = ph % NST;
           const int ahead = page_of(c + 1), p0 = first + c * kUChunk;
-          if (ph >= NST) wait_one(&bar.raw_free[is_v][rs], (ph / NST - 1) & 1);
+          // all four lanes or none, so that a stage that one has copies for completes
+          if (!__all_sync(0xFu, ph < NST || wait_one(&bar.raw_free[is_v][rs], (ph / NST - 1) & 1))) break;
           const bool there = page >= 0 && page < a.p.n_pages;
           const int have = there ? max(0, min(16, pc.len - p0)) : 0;
           held[is_v][rs][lane] = have;
@@ -722,6 +754,21 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
       __syncwarp();
       it += n;
       __syncthreads();
+      if (*abort_flag && c > 0) {  // products and copies in flight: of the last phases issued
+        const uint32_t last = it - n + c - 1;
+        auto settle = [&](uint64_t* b, uint32_t parity) {
+          for (uint32_t i = 0; i < kSettlePolls && !mbar_try_wait_for(b, parity, kSettleNs); ++i) {
+          }
+        };
+        if (gw < 2) {
+          settle(gw ? &bar.pv_done : &bar.k_free, last & 1);
+        } else {
+#pragma unroll 1
+          for (uint32_t k = 0; k < NST && k <= last; ++k)
+            settle(&bar.raw[gw == 3][(last - k) % NST], ((last - k) / NST) & 1);
+        }
+      }
+      __syncwarp();
     }
   }
   tc_fence_before();
