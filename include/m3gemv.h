@@ -482,8 +482,8 @@ M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint3
  * two f16 parts); large BF16 calls with more than 48 rows (tokens times query
  * heads per KV head) take the cached values rounded to f16, F16 ones V's (and
  * p in two parts).  That form hands tiles between warps, whose waits are bounded
- * ("attn_wait_us"): should one run out, the rows it was for become NaN and bit 0 of
- * the device status word is set.
+ * ("attn_wait_us"): should one run out, the rows it was for become NaN and
+ * kStatusAttnTimeout (64) is set in the device status word.
  * `workspace`: m3g_tree_attn_workspace() bytes (with the call's dtype, n_heads
  * and max_tokens) of device memory, 16-byte aligned, contents free, used by
  * one call at a time. */
@@ -512,8 +512,10 @@ M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t 
 /* Error word the kernels of `device` set when a bounded wait gives up
  * (bit 0: a staged-copy wait timed out; bit 3, value 8: a wait for a counter
  * bumped by another GPU or producer ran out, see "peer_wait_us"; bits 4 and 5,
- * values 16 and 32: a serving operator met a batch or page outside its limits).
- * clear != 0 resets it.  Synchronises the device. */
+ * values 16 and 32: a serving operator met a batch or page outside its limits;
+ * bit 6, value 64: a wait inside attention ran out).  The bits of the serving
+ * operators stay until they are reset here: no other call reports or clears
+ * them.  clear != 0 resets the word.  Synchronises the device. */
 M3G_API int m3g_device_status(int device, uint32_t* out, int clear);
 
 /* Number of kernel launches this library has enqueued in this process. */

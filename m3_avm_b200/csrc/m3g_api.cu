@@ -115,7 +115,7 @@ struct DevState {
   int sms = 0;
   int smem_per_sm = 0;
   int smem_optin = 0;
-  uint32_t* status = nullptr;
+  uint32_t* status = nullptr;  // of the GEMVs and the decoders; the serving operators' word lies kServeWord behind it
   // Set only in a per-call copy: the tensor-core GEMV's last CTA stores the
   // status word to *status_host (mapped host memory), counting CTAs in *fin_cnt.
   uint32_t* status_host = nullptr;
@@ -736,6 +736,11 @@ int status_word(int device, uint32_t** out) {
   *out = ds->status;
   return M3G_OK;
 }
+int serve_status_word(int device, uint32_t** out) {
+  if (int rc = status_word(device, out)) return rc;
+  *out += kServeWord;
+  return M3G_OK;
+}
 
 // y[out] = W x on `st` for device pointers, on `device` (the current one).
 int gemv_device(int device, uint32_t dtype, const uint8_t* w, uint64_t raw_len, const float* x, float* y,
@@ -1022,12 +1027,12 @@ int m3g_device_status(int device, uint32_t* out, int clear) {
   int prev = 0;
   M3G_CUDA(cudaGetDevice(&prev));
   M3G_CUDA(cudaSetDevice(device));
-  uint32_t s = 0;
-  cudaError_t e = cudaMemcpy(&s, ds->status, sizeof s, cudaMemcpyDeviceToHost);
+  uint32_t s[m3g::kServeWord + 1] = {};
+  cudaError_t e = cudaMemcpy(s, ds->status, sizeof s, cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && clear) e = cudaMemset(ds->status, 0, sizeof s);
   cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "m3g_device_status");
-  if (out) *out = s;
+  if (out) *out = s[0] | s[m3g::kServeWord];
   return M3G_OK;
 }
 

@@ -13,7 +13,11 @@ enum : uint32_t {
   kStatusPeerTimeout = 8u,  // a wait for other GPUs' rows gave up
   kStatusBadBatch = 16u,    // a sequence of a serving batch outside the call's limits (skipped)
   kStatusBadPage = 32u,     // a page id outside the cache pool (not accessed)
+  kStatusAttnTimeout = 64u, // a wait inside attention gave up (its rows are NaN)
 };
+// The serving operators report into a word of their own: the GEMVs' and the
+// decoders' calls look at theirs, and clear it whole, when they end.
+constexpr int kServeWord = 32;  // in 32-bit words behind the other
 
 constexpr int kMaxPeers = 8;  // ranks one decoder exchanges rows with (itself included)
 
@@ -169,6 +173,8 @@ bool decode_shard_ffn_enabled();
 
 // The per-device status word the kernels set kStatus* bits in.
 int status_word(int device, uint32_t** out);
+// The serving operators' word.
+int serve_status_word(int device, uint32_t** out);
 
 // Batched Q4_K GEMV, up to 8 columns of X per launch (m3g_mma.cu).
 constexpr int kGemm8Cols = 8;

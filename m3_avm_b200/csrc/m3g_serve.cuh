@@ -128,10 +128,10 @@ inline bool rows_aligned(const void* p, int64_t token_stride, int64_t head_strid
 // A pointer that is not a multiple of its elements' size (an access would fault).
 inline bool misaligned(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
 
-// The current device and its status word.
+// The current device and its status word for these operators.
 inline int serve_device(int* dev, uint32_t** status) {
   if (cudaGetDevice(dev) != cudaSuccess) return host_fail(M3G_ECUDA, "no CUDA device");
-  return status_word(*dev, status);
+  return serve_status_word(*dev, status);
 }
 inline cudaStream_t serve_stream(void* stream) {
   return stream ? static_cast<cudaStream_t>(stream) : cudaStreamLegacy;

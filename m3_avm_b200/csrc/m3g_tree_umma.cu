@@ -42,7 +42,7 @@
 // (weights written over them) and O.
 //
 // Every wait is bounded (wait_polls polls of wait_ns at most).  A role whose wait
-// gives up raises the copy-timeout bit and the CTA's abort word, which ends the
+// gives up raises the attention-timeout bit and the CTA's abort word, which ends the
 // others' waits, and neither issues nor arrives any more: a phase that a barrier
 // completes is always one whose work was done.  At the end of the piece the issuing
 // warps wait (bounded too) for their products and copies in flight; the rows of
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
     uint32_t polls = 0;
     while (!mbar_try_wait_for(b, parity, a.wait_ns)) {
       if (++polls < a.wait_polls && !*abort_flag) continue;
-      if (!*abort_flag) atomicOr(a.p.status, kStatusCopyTimeout);
+      if (!*abort_flag) atomicOr(a.p.status, kStatusAttnTimeout);
       *abort_flag = 1;
       return false;
     }
