@@ -10,7 +10,9 @@ device by default), enqueued without waiting, and raises M3GError for what the
 library refuses.  Given another stream than the current one, a call expects
 its inputs to be ready there; results and workspaces that it allocates are
 that stream's memory, kept until the current stream's work on them is done
-too, and whoever reads them elsewhere waits for the stream first.
+too, and whoever reads them elsewhere waits for the stream first.  Autograd
+does not see the calls: a tensor that requires a gradient is refused while
+gradients are recorded, since the gradient would be lost without a word.
 """
 from __future__ import annotations
 
@@ -73,11 +75,17 @@ def _fail(msg):
     raise _lib.M3GError(_lib.M3G_EINVAL, msg)
 
 
+def _check_no_grad(name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(f"{name} requires a gradient, which this call does not record: torch.no_grad() or detach()")
+
+
 def _check_rows(name, t, device=None, heads=None, head_dim=None, tokens=None):
     """t is (tokens, heads, head_dim) with a contiguous last dimension on `device`; returns its shape and strides."""
     shape = t.shape
     if len(shape) != 3:
         _fail(f"{name}: (tokens, heads, head_dim) is wanted, got {tuple(shape)}")
+    _check_no_grad(name, t)
     strides = t.stride()
     if strides[2] != 1 and shape[2] > 1:
         _fail(f"{name}: the last dimension has to be contiguous")
@@ -121,8 +129,8 @@ def _check_ints(name, t, device, shape):
 
 
 class Rope:
-    """A plan of rotary positions (m3g_rope_config); host arithmetic, usable on every device.  Autograd does not see
-    the calls: the gradient of apply(...) is apply(..., inverse=True) of the results' gradients."""
+    """A plan of rotary positions (m3g_rope_config); host arithmetic, usable on every device.  The gradient of
+    apply(...) is apply(..., inverse=True) of the results' gradients."""
 
     def __init__(self, head_dim: int, rot_dim: int | None = None, theta: float = 10000.0, interleaved: bool = False,
                  scaling: str = "none", factor: float = 1.0, orig_ctx: int = 0, low_freq: float = 1.0,

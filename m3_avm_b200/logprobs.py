@@ -5,7 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 from . import _lib
-from .attention import _call, _check_ints, _device, _fail, _on, act_dtype
+from .attention import _call, _check_ints, _check_no_grad, _device, _fail, _on, act_dtype
 
 
 class TokenLogprobs(NamedTuple):
@@ -27,6 +27,7 @@ def token_logprobs(logits, tokens=None, n_top: int = 0, entropy: bool = False, s
         _fail(f"{n_top} alternatives (at most 32)")
     rows, vocab = logits.shape
     device, dtype = _device(logits), act_dtype(logits)
+    _check_no_grad("logits", logits)
     n = 0
     lp = ent = ids = tops = None
     if tokens is not None:

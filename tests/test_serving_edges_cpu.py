@@ -117,3 +117,31 @@ def test_attention_bounds_that_are_and_are_not_too_large():
         assert call(1 << 20, 1 << 20, 1, 1 << 20, dtype) == _lib.M3G_EINVAL
         assert call(4096, 1 << 24, 1 << 12, 1 << 20, dtype) == _lib.M3G_EINVAL
         assert call(1, 1 << 30, 1 << 30, 64, dtype) == _lib.M3G_EINVAL
+
+
+def test_tensors_that_require_a_gradient_are_refused(monkeypatch):
+    """Autograd sees none of the calls: the gradient would be lost (in place, a leaf changed behind its back)."""
+    dev = Streams(monkeypatch)
+    cache = A.KvCache(8, 1, 2, 64, 16, 4, pool=torch.zeros(4 * 2 * 16 * 2 * 68, dtype=torch.uint8))
+    batch, rope = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64), A.Rope(64)
+    leaf = lambda *s: torch.randn(*s, requires_grad=True)  # noqa: E731
+    q, k, x = leaf(3, 4, 64), leaf(3, 2, 64), leaf(3, 40)
+    calls_of = [
+        lambda q, k, x: rope.apply(i32(3), q, k.detach()),
+        lambda q, k, x: rope.apply(i32(3), q.detach(), k),
+        lambda q, k, x: rope.apply(i32(3), q.detach(), q_out=q),
+        lambda q, k, x: cache.write(0, k, k.detach(), batch),
+        lambda q, k, x: cache.write(0, k.detach(), k, batch),
+        lambda q, k, x: A.tree_attention(q, cache, 0, batch),
+        lambda q, k, x: L.token_logprobs(x, n_top=2),
+    ]
+    for call in calls_of:
+        with pytest.raises(M3GError, match="gradient"):
+            call(q, k, x)
+    assert not dev.launched
+    with torch.no_grad():
+        for call in calls_of:
+            call(q, k, x)
+    for call in calls_of:
+        call(q.detach(), k.detach(), x.detach())
+    assert len(dev.launched) == 2 * len(calls_of)
