@@ -227,7 +227,12 @@ class KvCache:
         self.device = pool.get_device()
         self._workspace_bytes: dict[int, int] = {}
 
+    def _check_layer(self, layer):
+        if not 0 <= layer < self.n_layers:  # here: the library would get its low 32 bits
+            _fail(f"layer {layer} of {self.n_layers}")
+
     def _io(self, fn, layer, k, v, batch, stream):
+        self._check_layer(layer)
         device, dtype = _device(self.pool), act_dtype(k)
         if k.dtype is not v.dtype:
             _fail("k and v have one type")
@@ -257,9 +262,13 @@ class KvCache:
     def attention_workspace(self, n_heads: int, dtype=None, max_tokens: int = 1) -> int:
         """Bytes of workspace that attention of n_heads query heads of `dtype` (f32 by default) over at most max_tokens
         new tokens of a sequence needs."""
-        key = (n_heads, _dtypes.get(dtype, 0), max_tokens)
+        number = 0 if dtype is None else _dtypes.get(dtype)
+        key = (n_heads, number, max_tokens)
         got = self._workspace_bytes.get(key)
         if got is None:
+            if number is None:
+                _fail(f"attention of type {dtype} (f32, f16 and bf16 are supported)")
+            _check_sizes("attention", n_heads, max_tokens)
             need = ctypes.c_uint64()
             _lib.check(_lib.load().m3g_tree_attn_workspace(ctypes.byref(self.layout), key[1], n_heads, max_tokens,
                                                            ctypes.byref(need)))
@@ -275,6 +284,7 @@ def tree_attention(q, cache: KvCache, layer: int, batch: KvBatch, mask=None, sca
     at a time (allocated here when None)."""
     if scale is not None and not ctypes.c_float(scale).value > 0:  # in 32 bits, where 0 stands for the default
         _fail("scale must be positive")
+    cache._check_layer(layer)
     device, dtype = _device(q), act_dtype(q)
     shape, sq = _check_rows("q", q, cache.device, None, cache.head_dim, batch.n_tokens)
     heads = shape[1]

@@ -90,6 +90,8 @@ class GpuDecoder:
     def score(self, tokens, n_top: int = 0) -> TokenLogprobs:
         """prefill_logits(tokens) with, for each position i, the log probability of the token that follows it (tokens[i +
         1]; for the last position the greedy pick), the entropy and the n_top <= 32 most probable ids there."""
+        if not 0 <= n_top <= 32:
+            raise _lib.M3GError(_lib.M3G_EINVAL, f"{n_top} alternatives (at most 32)")
         t = np.ascontiguousarray(tokens, dtype=np.uint32)
         lp, ent = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
         ids = np.empty((t.size, n_top), np.uint32) if n_top > 0 else None

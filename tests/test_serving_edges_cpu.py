@@ -145,3 +145,23 @@ def test_tensors_that_require_a_gradient_are_refused(monkeypatch):
     for call in calls_of:
         call(q.detach(), k.detach(), x.detach())
     assert len(dev.launched) == 2 * len(calls_of)
+
+
+def test_numbers_past_32_bits_are_refused_not_cut(monkeypatch):
+    from m3_avm_b200.decoder import GpuDecoder
+
+    dev = Streams(monkeypatch)
+    cache = A.KvCache(8, 2, 2, 64, 16, 4, pool=torch.zeros(2 * 4 * 2 * 16 * 2 * 68, dtype=torch.uint8))
+    batch, q, k = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64), torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
+    for layer in (2, -1, 2 ** 32, 2 ** 32 + 1, -2 ** 32):
+        for call in (lambda: cache.write(layer, k, k, batch), lambda: cache.read(layer, batch),
+                     lambda: A.tree_attention(q, cache, layer, batch)):
+            with pytest.raises(M3GError, match="layer"):
+                call()
+    assert not dev.launched
+    for args in ((2 ** 32 + 4, None, 1), (4, None, 2 ** 32 + 1), (4, None, -1), (4, torch.float64, 1)):
+        with pytest.raises(M3GError):
+            cache.attention_workspace(*args)
+    for n_top in (-1, 33, 2 ** 32 + 1):
+        with pytest.raises(M3GError, match="alternatives"):
+            GpuDecoder.score(GpuDecoder.__new__(GpuDecoder), [], n_top=n_top)
