@@ -128,7 +128,19 @@ def _check_ints(name, t, device, shape):
         _fail(f"{name}: a contiguous int32 tensor of shape {shape} on the device of the other tensors is wanted")
 
 
-class Rope:
+class _Told:
+    """What the library was told once, by value and by address: public attributes stay as they were made.  (A changed
+    n_tokens would pass the checks of the tensors here, and the kernels would still go by the old one.)"""
+
+    _done = False
+
+    def __setattr__(self, name, value):
+        if self._done and not name.startswith("_"):
+            _fail(f"{type(self).__name__}.{name} cannot be changed: make a new {type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+
+class Rope(_Told):
     """A plan of rotary positions (m3g_rope_config); host arithmetic, usable on every device.  The gradient of
     apply(...) is apply(..., inverse=True) of the results' gradients."""
 
@@ -146,6 +158,7 @@ class Rope:
         h = ctypes.c_void_p()
         _lib.check(_lib.load().m3g_rope_create(ctypes.byref(cfg), ctypes.byref(h)))
         self._h = h
+        self._done = True
 
     def apply(self, positions, q, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
         """Turns q and k (k may be None) at int32 `positions` (tokens,); q_out, k_out may be q and k themselves.
@@ -185,7 +198,7 @@ class Rope:
             pass
 
 
-class KvBatch:
+class KvBatch(_Told):
     """The new tokens of a batch of sequences (m3g_kv_batch).  `q_start` (n + 1,), `ctx_len` (n,) and `page_table`
     (n, max_pages) are int32 tensors of the GPU, read when an operator runs (a captured step replays with what they
     hold then); max_tokens and max_len bound what they may say."""
@@ -203,9 +216,10 @@ class KvBatch:
         self.n_tokens, self.max_tokens, self.max_len = n_tokens, max_tokens, max_len
         self.args = _lib.KvBatchArgs(q_start.data_ptr(), ctx_len.data_ptr(), page_table.data_ptr(), n,
                                      page_table.shape[1], n_tokens, max_tokens, max_len)
+        self._done = True
 
 
-class KvCache:
+class KvCache(_Told):
     """A paged cache of K and V rows in Q8_0 or Q4_0 blocks (m3g_kv_layout).  Its memory is one uint8 tensor, `pool`,
     allocated here (zeros) or the caller's own."""
 
@@ -225,7 +239,8 @@ class KvCache:
             _fail(f"the pool: a contiguous uint8 tensor of {need.value} bytes is wanted")
         self.pool = pool
         self.device = pool.get_device()
-        self._workspace_bytes: dict[int, int] = {}
+        self._workspace_bytes: dict[tuple, int] = {}
+        self._done = True
 
     def _check_layer(self, layer):
         if not 0 <= layer < self.n_layers:  # here: the library would get its low 32 bits

@@ -165,3 +165,17 @@ def test_numbers_past_32_bits_are_refused_not_cut(monkeypatch):
     for n_top in (-1, 33, 2 ** 32 + 1):
         with pytest.raises(M3GError, match="alternatives"):
             GpuDecoder.score(GpuDecoder.__new__(GpuDecoder), [], n_top=n_top)
+
+
+def test_what_the_library_was_told_cannot_be_changed_behind_its_back():
+    cache = A.KvCache(8, 1, 2, 64, 16, 4, pool=torch.zeros(4 * 2 * 16 * 2 * 68, dtype=torch.uint8))
+    batch, rope = A.KvBatch(i32(2), i32(1), i32(1, 4), 3, 3, 64), A.Rope(64)
+    for obj, name, value in ((batch, "n_tokens", 5), (batch, "ctx_len", i32(1)), (batch, "max_len", 128),
+                             (cache, "pool", torch.zeros(16, dtype=torch.uint8)), (cache, "n_layers", 9),
+                             (rope, "head_dim", 128)):
+        before = getattr(obj, name)
+        with pytest.raises(M3GError, match="cannot be changed"):
+            setattr(obj, name, value)
+        assert getattr(obj, name) is before
+    batch.ctx_len[0] = 7  # the contents are the caller's
+    rope.close()
