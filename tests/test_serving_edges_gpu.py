@@ -227,3 +227,22 @@ def test_sequences_that_overlap_past_all_bounds_are_refused_whole(dtype):
     tree_attention(q, cache, 0, batch, out=out)
     assert status() == 16
     assert bool((out == 5).all())
+
+
+# ---------------------------------------------------------------- log probabilities of rows that few threads hold
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab,k", [(700, 3500, 32), (1, 3500, 32), (300, 2100, 32), (300, 1031, 20), (40, 259, 32),
+                                          (40, 250, 32), (700, 1800, 32)])
+def test_logprobs_of_short_rows_with_many_alternatives(dtype, rows, vocab, k):
+    from m3_avm_b200.logprobs import token_logprobs
+    from tests.test_serving_gpu import logprob_reference, lp_tolerance
+
+    x = randn(rows + vocab, rows, vocab, scale=4.0, dtype=dtype)
+    tokens = torch.randint(0, vocab, (rows, 1), dtype=torch.int32, generator=torch.Generator().manual_seed(1))
+    got = token_logprobs(x, tokens.cuda(), n_top=k, entropy=True)
+    given, entropy, ids, tops = logprob_reference(x.cpu(), tokens, k)
+    tol, etol = lp_tolerance(x.cpu())
+    assert torch.equal(got.top_ids.cpu().long(), ids)
+    assert bool(((got.top_logprobs.double().cpu() - tops).abs() <= tol).all())
+    assert bool(((got.logprob.double().cpu() - given).abs() <= tol).all())
+    assert bool(((got.entropy.double().cpu() - entropy).abs() <= etol).all())
