@@ -246,3 +246,94 @@ def test_logprobs_of_short_rows_with_many_alternatives(dtype, rows, vocab, k):
     assert bool(((got.top_logprobs.double().cpu() - tops).abs() <= tol).all())
     assert bool(((got.logprob.double().cpu() - given).abs() <= tol).all())
     assert bool(((got.entropy.double().cpu() - entropy).abs() <= etol).all())
+
+
+# ---------------------------------------------------------------- the pool's layout, byte by byte
+def host_blocks(rows, dtype):
+    """Codes and scales (as bytes) of rows (..., head_dim) by the library's host quantisers."""
+    from m3_avm_b200 import quant
+
+    x = rows.float().cpu().numpy()
+    codes, scales = [], []
+    for row in x.reshape(-1, x.shape[-1]):
+        c, s = b"", b""
+        for b in row.reshape(-1, 32):
+            dst = bytearray(34 if dtype == 8 else 18)
+            assert (quant.quantize_q8_0 if dtype == 8 else quant.quantize_q4_0)(np.ascontiguousarray(b), dst)
+            s += bytes(dst[:2])
+            body = np.frombuffer(bytes(dst[2:]), np.uint8)
+            c += (body + 128).astype(np.uint8).tobytes() if dtype == 8 else body.tobytes()
+        codes.append(np.frombuffer(c, np.uint8))
+        scales.append(np.frombuffer(s, np.uint8))
+    shape = x.shape[:-1] + (-1,)
+    return np.stack(codes).reshape(shape), np.stack(scales).reshape(shape)
+
+
+@pytest.mark.parametrize("dtype", [8, 2])
+@pytest.mark.parametrize("kvh,hd,page", [(3, 128, 16), (2, 64, 32), (40, 64, 16)])
+def test_pool_bytes_are_those_of_the_documented_layout(dtype, kvh, hd, page):
+    """Every byte of a pool of 3 layers: [K codes, K scales, V codes, V scales][page][head][place], others untouched."""
+    from m3_avm_b200.attention import KvCache
+
+    ctx, new, layers, layer = [5, 0, page - 1, 40], [7, 1, page + 2, 0], 3, 1
+    batch, pages, table, _ = R.make_batch(ctx, new, page, seed=kvh)
+    cache = KvCache(dtype, layers, kvh, hd, page, pages)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache.pool.copy_(torch.randint(0, 256, cache.pool.shape, generator=g, device="cuda", dtype=torch.uint8))
+    want = cache.pool.cpu().numpy().copy()
+    k, v = randn(1, sum(new), kvh, hd, scale=2.0), randn(2, sum(new), kvh, hd, scale=0.1)
+    cache.write(layer, k, v, batch)
+    cb, sb = (hd if dtype == 8 else hd // 2), hd // 16
+    rows = pages * kvh * page
+    base = layer * rows * 2 * (cb + sb)
+    at = {"kc": base, "ks": base + rows * cb, "vc": base + rows * (cb + sb), "vs": base + rows * (2 * cb + sb)}
+    for x, c, s in ((k, "kc", "ks"), (v, "vc", "vs")):
+        codes, scales = host_blocks(x, dtype)
+        t = 0
+        for i, (before, n) in enumerate(zip(ctx, new)):
+            for pos in range(before, before + n):
+                for h in range(kvh):
+                    row = (int(table[i, pos // page]) * kvh + h) * page + pos % page
+                    want[at[c] + row * cb:at[c] + (row + 1) * cb] = codes[t, h]
+                    want[at[s] + row * sb:at[s] + (row + 1) * sb] = scales[t, h]
+                t += 1
+    assert np.array_equal(cache.pool.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+def test_cache_values_below_zero_that_are_not_finite_or_too_large(q8):
+    from m3_avm_b200.attention import KvCache
+
+    batch, pages, _, _ = R.make_batch([0], [8], 16)
+    cache = KvCache(8 if q8 else 2, 1, 1, 64, 16, pages)
+    x = randn(3, 8, 1, 64)
+    x[0, 0, 3], x[1, 0, 40], x[2, 0, 31], x[3, 0, 5] = float("nan"), float("inf"), float("-inf"), 3e38
+    x[4, 0, 5], x[5, 0, 5], x[6] = 65504.0 * (127 if q8 else 7), 1e-45, 1e-40
+    cache.write(0, x, -x, batch)
+    for got, given in zip(cache.read(0, batch), (x, -x)):
+        want = R.quantised(given, q8)
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+        assert torch.equal(got.cpu().nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (F16, 128), (F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("ksize,vsize", [(1e5, 1.0), (1.0, 1e4), (1e5, 1e4)])
+def test_attention_large_form_of_scales_past_the_f16_range(dtype, hd, q8, ksize, vsize):
+    """Some blocks whose scales are past 500 (K's scores with an attention scale that keeps them in range)."""
+    from m3_avm_b200.attention import KvCache, tree_attention
+
+    batch, pages, _, _ = R.make_batch([200], [6], 16)
+    cache = KvCache(8 if q8 else 2, 1, 1, hd, 16, pages)
+    full = R.whole(batch, [200], [6])
+    k, v = randn(1, 206, 1, hd), randn(2, 206, 1, hd)
+    k[60:100] *= ksize
+    v[90:150] *= vsize if q8 else vsize / 2
+    cache.write(0, k, v, full)
+    q = randn(3, 6, 64, hd, dtype=dtype)
+    scale = 0.05 / ksize
+    got = tree_attention(q, cache, 0, roomy(batch, 16), scale=scale)
+    bits = [np.tril(np.ones((6, 6), bool))]
+    want, vmax, smag = R.attention(q, [R.quantised(k, q8).double()], [R.quantised(v, q8).double()], [200], [6], bits,
+                                   scale)
+    assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
