@@ -163,7 +163,7 @@ __device__ __forceinline__ void find_places(const KvIoArgs& a, int t0, int n_tok
       else hi = mid;
     }
     long long at = -1;
-    bool bad = false;
+    bool bad = false;  // hold_starts reports it
     const SeqView s = seq_view(a.b, a.cap, lo, &bad);
     if (t >= s.q0 && t - s.q0 < s.n) {
       const int pos = s.ctx + (t - s.q0);
@@ -173,16 +173,25 @@ __device__ __forceinline__ void find_places(const KvIoArgs& a, int t0, int n_tok
       else
         atomicOr(a.p.status, kStatusBadPage);
     }
-    if (bad) atomicOr(a.p.status, kStatusBadBatch);
     place[tid] = at;
   }
   __syncthreads();
 }
 
+// The starts into shared memory; the first CTA reports sequences outside the call's
+// limits, also those that no token leads to.
 __device__ __forceinline__ void hold_starts(const KvIoArgs& a, int32_t* starts) {
   const int n_seqs = static_cast<int>(a.b.n_seqs);
-  if (n_seqs <= kKvStarts)
-    for (int i = threadIdx.x; i < n_seqs; i += kKvThreads) starts[i] = a.b.q_start[i];
+  bool bad = false;
+  if (blockIdx.x == 0) {
+    for (int s = threadIdx.x; s < n_seqs; s += kKvThreads) {
+      const SeqView v = seq_view(a.b, a.cap, s, &bad);
+      if (n_seqs <= kKvStarts) starts[s] = v.q0;
+    }
+  } else if (n_seqs <= kKvStarts) {
+    for (int s = threadIdx.x; s < n_seqs; s += kKvThreads) starts[s] = a.b.q_start[s];
+  }
+  if (bad) atomicOr(a.p.status, kStatusBadBatch);
   __syncthreads();
 }
 

@@ -337,3 +337,28 @@ def test_attention_large_form_of_scales_past_the_f16_range(dtype, hd, q8, ksize,
     want, vmax, smag = R.attention(q, [R.quantised(k, q8).double()], [R.quantised(v, q8).double()], [200], [6], bits,
                                    scale)
     assert_within(got, want, R.attention_bound(want, vmax, smag, dtype))
+
+
+# ---------------------------------------------------------------- batches that say something wrong
+@pytest.mark.parametrize("q_start,ctx", [
+    ([0, 6, 3, 9], [0, 0, 0]),    # starts that go back
+    ([0, 9, 9, 11], [0, 0, 0]),   # a sequence behind the tensors' rows
+    ([0, 4, 4, 9], [0, -1, 0]),   # a context of less than nothing, without new tokens
+    ([-2, 0, 5, 9], [0, 0, 0]),   # a start before the first row
+])
+def test_every_operator_reports_every_bad_sequence(q_start, ctx):
+    from m3_avm_b200.attention import KvBatch, KvCache, tree_attention
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    cache = KvCache(8, 1, 2, 64, 16, 3)
+    batch = KvBatch(i32(q_start), i32(ctx), i32([[0], [1], [2]]), 9, 9, 16)
+    x = randn(1, 9, 2, 64)
+    cache.write(0, x, x, batch)
+    assert status() == 16
+    k = torch.full_like(x, 7.0)
+    cache.read(0, batch, k_out=k, v_out=torch.full_like(x, 7.0))
+    assert status() == 16
+    tree_attention(randn(2, 9, 4, 64), cache, 0, batch)
+    assert status() == 16
+    last = slice(q_start[2], min(q_start[3], 9)) if q_start[3] <= 9 else slice(9, 9)
+    assert torch.equal(k[last].cpu(), R.quantised(x[last], True))
