@@ -357,12 +357,52 @@ __global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(
           const uint2 x = *reinterpret_cast<const uint2*>(vscales + (8 * nt + 2 * t) * St::SB);
           dv[nt][0] = x.x; dv[nt][1] = x.y;
         }
+      }
+      if (tail) {
+        // A scale that is not finite among them (0 times it is NaN): the rows that see
+        // its position get NaN in its block of values, however small their weights, and
+        // the others are not to meet it.
+        const __half2 most = __half2half2(__ushort_as_half(0x7BFF));  // 65504
+        bool odd = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < NB; ++h) odd = odd || !__hble2(__habs2(*reinterpret_cast<const __half2*>(&dv[nt][h])), most);
+        if (__any_sync(0xFFFFFFFFu, odd)) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t vis = tree_sees(a, sw.v.q0, token[i], ctx, len, p0);
+            uint32_t blocks = 0u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int h = 0; h < 2 * NB; ++h) {  // position h / NB of the two, block h % NB
+                const uint32_t d = dv[nt][h / NB * (NB / 2) + h % NB / 2] >> (16 * (h & 1)) & 0x7FFFu;
+                if (d > 0x7BFFu && (vis >> (8 * nt + 2 * t + h / NB) & 1u)) blocks |= 1u << (h % NB);
+              }
+            blocks |= __shfl_xor_sync(0xFFFFFFFFu, blocks, 1);
+            blocks |= __shfl_xor_sync(0xFFFFFFFFu, blocks, 2);
+#pragma unroll
+            for (int b = 0; b < NO; ++b)
+              if (blocks >> (b / 4) & 1u) o[b][2 * i] = o[b][2 * i + 1] = NAN;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < NB; ++h) {
+              if ((dv[nt][h] & 0x7FFFu) > 0x7BFFu) dv[nt][h] &= 0xFFFF0000u;
+              if ((dv[nt][h] >> 16 & 0x7FFFu) > 0x7BFFu) dv[nt][h] &= 0x0000FFFFu;
+            }
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int h = 0; h < NB; ++h) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&dv[nt][h])));
       }
 #pragma unroll
       for (int x = 1; x < 4; x <<= 1) big = __hmax2(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-      const float dmax = fmaxf(__low2float(big), __high2float(big));
+      const float dmax = fminf(fmaxf(__low2float(big), __high2float(big)), 65504.f);  // an infinite one spoils its block alone
       float shrink = 1.f;
       if (dmax > dref) {  // the same for all lanes
         const float up = __uint_as_float((__float_as_uint(dmax) + 0x7FFFFFu) & 0x7F800000u);
@@ -416,11 +456,7 @@ __global__ void __launch_bounds__(kTreeThreads, (Ctas<HD>::kPerSm)) k_tree_attn(
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint64_t w = mul2(s2[nt][i], e);
-              float w0 = low(w), w1 = high(w);
-              if (tail) {  // a position that the row does not see adds nothing, NaN or not
-                w0 = low(s2[nt][i]) == 0.f ? 0.f : w0;
-                w1 = high(s2[nt][i]) == 0.f ? 0.f : w1;
-              }
+              const float w0 = low(w), w1 = high(w);
               const uint32_t hi = pack_f16(w0, w1);
               ph[2 * h + i] = hi;
               if (SPLIT) {

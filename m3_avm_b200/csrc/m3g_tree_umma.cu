@@ -143,6 +143,8 @@ __device__ __forceinline__ float2 two(uint32_t w) {
 template <class T>
 __device__ __forceinline__ T uniform(T v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
 
+__device__ __forceinline__ bool not_finite(__half d) { return (__half_as_ushort(d) & 0x7FFFu) > 0x7BFFu; }
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect() {
   uint32_t p;
@@ -233,8 +235,8 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
   __shared__ UPiece pc;
   __shared__ uint32_t tslot;
   __shared__ int abort_word;
-  // Of a chunk's groups of 16 positions: 1 K, 2 V at 2^-7, 4 NaN in V of a tail;
-  // and of a tail chunk's positions the blocks of V that are NaN.  Four chunks
+  // Of a chunk's groups of 16 positions: 1 K, 2 V at 2^-7, 4 a scale of V that is not
+  // finite in a tail; and of a tail chunk's positions the blocks of V with such scales.  Four chunks
   // deep: K is unpacked at most three ahead of a softmax that still reads.
   __shared__ __align__(16) int odd[4][4];
   __shared__ uint32_t v_nan[4][kUChunk];
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
             if (b / NB >= have) continue;
             const __half dv = sc[is_v ? b : 16 * NB + b];
             odd_k |= !is_v && __habs(sc[b]) > lim;
-            odd_v |= (__habs(dv) > lim ? 1 : 0) | (__hisnan(dv) ? 2 : 0);
+            odd_v |= (__habs(dv) > lim ? 1 : 0) | (not_finite(dv) ? 2 : 0);
           }
           flags = (__any_sync(0xFFFFFFFFu, odd_k) ? 1 : 0) | (__any_sync(0xFFFFFFFFu, odd_v & 1) ? 2 : 0) |
                   (__any_sync(0xFFFFFFFFu, odd_v & 2) && c >= first_tail ? 4 : 0);
@@ -626,16 +628,16 @@ __global__ void __launch_bounds__(kUThreads, 2) k_tree_umma(const __grid_constan
 #pragma unroll
           for (int j = 0; j < PPL; ++j) d[j] = __hmul(d[j], __float2half_rn(0x1p-7f));
         }
-        if (flags & 4) {  // a row that does not see a position must not meet its NaN: it is put back at the end
+        if (flags & 4) {  // a row that does not see a position must not meet 0 times it: NaN is put back at the end
           if (is_v) {
 #pragma unroll
             for (int j = 0; j < PPL; ++j)
-              if (__hisnan(d[j])) d[j] = __ushort_as_half(0);
+              if (not_finite(d[j])) d[j] = __ushort_as_half(0);
           } else if (lane < 16) {
             uint32_t blocks = 0u;
 #pragma unroll 1
             for (int b = 0; b < NB; ++b)
-              if (lane < have && __hisnan(sc[(16 + lane) * NB + b]))
+              if (lane < have && not_finite(sc[(16 + lane) * NB + b]))
                 blocks |= 1u << b;
             v_nan[ph & 3][16 * gw + lane] = blocks;
           }

@@ -362,3 +362,30 @@ def test_every_operator_reports_every_bad_sequence(q_start, ctx):
     assert status() == 16
     last = slice(q_start[2], min(q_start[3], 9)) if q_start[3] <= 9 else slice(9, 9)
     assert torch.equal(k[last].cpu(), R.quantised(x[last], True))
+
+
+@pytest.mark.parametrize("dtype,heads,large", [(F32, 4, False), (BF16, 4, False), (F16, 4, False), (BF16, 64, True),
+                                               (F16, 64, True)])
+@pytest.mark.parametrize("at", [3, 41])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_attention_a_seen_nan_counts_however_small_its_weight(dtype, heads, large, at, infinite):
+    """0 * NaN (or, in another writer's pool, an infinite scale): a position whose score is 2000 below the others', in the context and among the new tokens."""
+    from m3_avm_b200.attention import KvCache, tree_attention
+
+    batch, pages, _, _ = R.make_batch([40], [5], 16)
+    cache = KvCache(8, 1, 1, 64, 16, pages)
+    full = R.whole(batch, [40], [5])
+    k, v = randn(1, 45, 1, 64, scale=0.1), randn(2, 45, 1, 64)
+    q = randn(3, 1, 1, 64).sign().expand(5, heads, 64).to(dtype).contiguous()
+    k[at] = -40.0 * q[0, :1].float()
+    v[at, 0, 7] = float("nan")
+    cache.write(0, k, v, full)
+    if infinite:
+        scales = planes(cache)[3]
+        scales.copy_(torch.where(torch.isnan(scales), torch.tensor(float("inf"), dtype=F16, device="cuda"), scales))
+        assert int(torch.isinf(scales).sum()) == 1
+    got = tree_attention(q, cache, 0, roomy(batch, 16) if large else batch, scale=1.0)
+    seen = [max(at - 40, 0) <= j for j in range(5)]
+    for j in range(5):
+        assert bool(torch.isnan(got[j, :, :32]).all()) == seen[j]  # the block of 32 values that the NaN took with it
+        assert not bool(torch.isnan(got[j, :, 32:]).any())
