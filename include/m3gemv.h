@@ -378,13 +378,14 @@ M3G_API int m3g_matvec_greedy_noalloc(const float* x, const uint8_t* raw, uint64
  * device memory (`dtype` of each call); the last dimension is contiguous, the
  * other strides are in elements and free (not negative); pointers are multiples
  * of their elements' size (M3G_EINVAL otherwise).  Calls hold no state:
- * any number may run at once on different streams, and all can be captured. */
+ * any number may run at once on different streams, and all can be captured,
+ * the first one of a process too. */
 
 /* Rotary positions.  Pair i of a head, (x[i], x[i + rot_dim/2]), or (x[2i],
  * x[2i + 1]) when interleaved, turns by positions[token] * f_i with f_i =
  * theta^(-2i / rot_dim), scaled by `scaling`; elements from rot_dim on are
- * copied.  Angles are exact to 2^-50 of a turn at any 32-bit position
- * (negative ones turn backwards). */
+ * copied.  Angles are off by 2^-25 + |position| 2^-53 of a turn at most
+ * (negative positions turn backwards). */
 #define M3G_ROPE_NONE 0u
 #define M3G_ROPE_LINEAR 1u /* f_i / factor */
 #define M3G_ROPE_NTK 2u    /* theta * factor^(rot_dim / (rot_dim - 2)) */
@@ -423,10 +424,12 @@ M3G_API int m3g_rope_dev(const m3g_rope* rope, uint32_t dtype, const int32_t* po
  * [n_pages][n_kv_heads][page_size] rows of head_dim (Q4_0: head_dim/2) code
  * bytes, or of head_dim/32 f16 scales.  A Q8_0 code byte c stands for
  * (c - 128) * d; a Q4_0 row holds the 16-byte nibble groups of its blocks as
- * GGUF has them (low nibbles the first 16 values), n for (n - 8) * d. */
+ * GGUF has them (low nibbles the first 16 values), n for (n - 8) * d.  Scales
+ * that m3g_kv_write_dev stores are not negative; those of other writers may be. */
 typedef struct {
     uint32_t dtype;       /* M3G_DTYPE_Q8_0 or M3G_DTYPE_Q4_0 */
-    uint32_t n_layers, n_kv_heads;
+    uint32_t n_layers;    /* <= 4096 */
+    uint32_t n_kv_heads;  /* <= 1024 */
     uint32_t head_dim;    /* 64 or 128 */
     uint32_t page_size;   /* positions per page: a power of two, 16 .. 1024 */
     uint64_t n_pages;     /* < 2^31 */
@@ -437,17 +440,20 @@ M3G_API int m3g_kv_bytes(const m3g_kv_layout* layout, uint64_t* out);
  * q_start[s+1]-1 of the call's n_tokens, at positions ctx_len[s], ctx_len[s]+1,
  * ... of its pages page_table[s * max_pages + position / page_size] (device
  * memory throughout).  Pages may be shared by sequences that only read them.
- * The kernels check what they read: a sequence with more than max_tokens new
- * tokens, longer than max_len positions or than its max_pages pages, or with
- * starts outside [0, n_tokens], is skipped (its output rows stay as they
- * were) and sets kStatusBadBatch (16) in the device status word; a page
- * outside the pool is neither read nor written (its positions read as zeros)
- * and sets kStatusBadPage (32). */
+ * Starts do not decrease.  Rows of no sequence (behind the last one's) are not
+ * written by any call.  The kernels check what they read: a sequence with more
+ * than max_tokens new tokens or fewer than none, longer than max_len positions or
+ * than its max_pages pages, or with new tokens outside [0, n_tokens), is skipped
+ * (its output rows stay as they were) and sets kStatusBadBatch (16) in the device
+ * status word; a page outside the pool is neither read nor written and sets
+ * kStatusBadPage (32): attention takes its positions as zeros, m3g_kv_read_dev
+ * leaves their rows as they were. */
 typedef struct {
     const int32_t* q_start;    /* [n_seqs + 1] */
     const int32_t* ctx_len;    /* [n_seqs] */
     const int32_t* page_table; /* [n_seqs][max_pages] */
-    uint32_t n_seqs, max_pages;
+    uint32_t n_seqs;           /* <= 2^20 */
+    uint32_t max_pages;        /* row length of page_table */
     uint32_t n_tokens;         /* rows of the tensors of the call */
     uint32_t max_tokens;       /* most new tokens of one sequence */
     uint32_t max_len;          /* most positions of one sequence, new tokens included */
@@ -478,10 +484,16 @@ M3G_API int m3g_kv_read_dev(const m3g_kv_layout* layout, const void* pool, uint3
  * token that sees nothing gets zeros.  Query head h reads KV head h /
  * (n_heads / n_kv_heads).  scale 0 means 1 / sqrt(head_dim).  q and out are
  * [n_tokens][n_heads][head_dim] of `dtype`; `out` may be q itself.  Sums are
- * f32.  Products take the cached codes exactly and p as f16 (F32: q and p in
- * two f16 parts); large BF16 calls with more than 48 rows (tokens times query
- * heads per KV head) take the cached values rounded to f16, F16 ones V's (and
- * p in two parts).  That form hands tiles between warps, whose waits are bounded
+ * f32, exponentials good to 2^-22.  Products take the cached codes exactly and p
+ * times V's scale as f16 (F32: q and p in two f16 parts), relative to the largest
+ * scale at hand, so that a V a million times larger, seen or not, costs the others
+ * bits; large calls with many rows (the most tokens of a sequence times query heads
+ * per KV head: BF16 49, 65 with heads of 64; F16 81) take cached values rounded to
+ * f16 (F16: V's alone, and p in two parts).  A V scale that is not finite makes its
+ * block NaN or infinite in the rows that see it, not in others.  At most 32768 query
+ * heads; a batch that can come to 2^31 chunks (16 rows by 128 positions, or 128
+ * by 64) is refused, one whose arrays alone say so is skipped whole with
+ * kStatusBadBatch.  The form for many rows hands tiles between warps, whose waits are bounded
  * ("attn_wait_us"): should one run out, the rows it was for become NaN and
  * kStatusAttnTimeout (64) is set in the device status word.
  * `workspace`: m3g_tree_attn_workspace() bytes (with the call's dtype, n_heads
@@ -495,13 +507,14 @@ M3G_API int m3g_tree_attn_dev(const m3g_kv_layout* layout, const void* pool, uin
                               void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Log probabilities of given tokens, lp = x_t - lse(x), of each row of
- * logits [rows][vocab]: tokens [rows][n_tokens] -> logprob [rows][n_tokens]
- * (-inf for an id outside the vocabulary); entropy [rows] of the row's
+ * logits [rows][vocab] (rows <= 2^27, vocab <= 2^30): tokens [rows][n_tokens],
+ * n_tokens <= 512, -> logprob [rows][n_tokens] (-inf for an id outside the vocabulary); entropy [rows] of the row's
  * distribution unless NULL; the n_top (<= 32) most probable ids, ties to the
  * lowest id, with their log probabilities, [rows][n_top] each.  Logits of
  * -inf have probability 0.  A row with a NaN, a +inf or nothing above -inf
  * has no distribution: its numbers are NaN (its ids rank NaN below -inf).
- * tokens, top_id may be NULL with n_tokens, n_top 0.  Sums are f32. */
+ * tokens, top_id may be NULL with n_tokens, n_top 0.  Sums are f32 of
+ * exponentials good to 2^-22. */
 M3G_API int m3g_token_logprobs_dev(uint32_t dtype, const void* logits, uint64_t rows, uint64_t vocab,
                                    int64_t row_stride, const int32_t* tokens, uint32_t n_tokens, float* logprob,
                                    float* entropy, uint32_t n_top, int32_t* top_id, float* top_logprob,

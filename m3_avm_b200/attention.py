@@ -10,7 +10,11 @@ device by default), enqueued without waiting, and raises M3GError for what the
 library refuses.  Given another stream than the current one, a call expects
 its inputs to be ready there; results and workspaces that it allocates are
 that stream's memory, kept until the current stream's work on them is done
-too, and whoever reads them elsewhere waits for the stream first.  Autograd
+too, and whoever reads them elsewhere waits for the stream first.  What the
+kernels skip on the device (a sequence past the batch's limits, a page outside
+the pool, a wait that ran out) raises nothing: matvec_quant.device_status says
+so, and the rows stay as they were, which in a result allocated by the call,
+as in its rows of no sequence, is whatever its memory held.  Autograd
 does not see the calls: a tensor that requires a gradient is refused while
 gradients are recorded, since the gradient would be lost without a word.
 """

@@ -16,10 +16,11 @@
 // share of the tokens, 64 at a time, whose places its threads look up first, one
 // token each.
 //
-// Measured: 30000 BF16 tokens of 8 heads of 128 to Q4_0, written 42 us (3.8 TB/s of
-// what it must move), read back 26 us (6.1 TB/s); 36873 tokens to Q8_0 and back
-// as one pair 63 us.  Writing is bound by issue: some 115 instructions for a
-// thread's 8 values.
+// Measured: 20954 BF16 tokens of 8 + 8 heads of 128 (5 ragged prompts) to Q4_0, written
+// 38.7 us (110 MB, 2.8 TB/s), read back 24.2 us (4.5 TB/s); 23918 tokens to Q8_0
+// 34.2 us (150 MB, 4.4 TB/s) and back 32.4 us (4.6 TB/s).  Issue slots are 70 % used
+// in writing (125 instructions for a thread's 8 values to Q8_0, 167 to Q4_0, where 29 %
+// of the warps hold a value near a border), 64 % in reading (87).
 #include <algorithm>
 
 #include "m3g_device.cuh"

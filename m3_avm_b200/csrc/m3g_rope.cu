@@ -2,10 +2,11 @@
 //
 // Pair i of a token at position p turns by the angle p * f_i.  The plan holds
 // f_i / 2pi as a 64-bit fraction of a turn, so p * f_i modulo one turn is one
-// wrapping 64-bit integer product, exact to p * 2^-53 of f_i's own rounding:
-// no range reduction, and far positions lose nothing (an f32 product is off by
-// 0.06 rad at position 10^6).  sincospif of the top 32 bits gives cos and sin
-// once per token; all its heads share them through shared memory.
+// wrapping 64-bit integer product without a range reduction.  What it is off by: f_i
+// is a double, right to some units (|p| 2^-53 turns); the product's top 32 bits become
+// sincospif's f32 argument (2^-26 turns).  An f32 product is off by 0.06 rad at
+// position 10^6 already.  cos and sin are worked out once per token; all its heads
+// share them through shared memory.
 //
 // Bound: HBM (each element read and written once; 16384 BF16 tokens of 72 heads of 128
 // 116 us, 5.2 TB/s; 4099 F32 tokens of 40 heads of 64 14.5 us, 5.8 TB/s).  A CTA takes a run of tokens.

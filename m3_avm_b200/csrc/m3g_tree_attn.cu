@@ -28,10 +28,10 @@
 // (maximum, sum, results) in the workspace for k_tree_join.
 //
 // Bound.  With few rows HBM: 48 ragged contexts of up to 16000 positions, 4 rows
-// a KV head, BF16 over Q8_0: 245 us, 4.6 TB/s; the same loads without the
-// arithmetic take 181 us, the rest is ALU work (unpacking, softmax) beside them.
-// One context of 1024 positions: 9.3 us, of which a launch, the loads' latency
-// and the join each take 2 to 3.
+// a KV head, BF16 over Q8_0: 239 us in a graph, 4.75 TB/s (one call after another from
+// Python 268); the same loads without the arithmetic take 181 us, the rest is ALU
+// work (unpacking, softmax) beside them.  One context of 1024 positions: 9.2 to 9.6 us,
+// of which a launch, the loads' latency and the join each take 2 to 3.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -585,13 +585,16 @@ cudaError_t launch_tree_t(const TreeArgs& a, bool q8, int sms, cudaStream_t st) 
 // Which form: the one of 128-row tiles (m3g_tree_umma.cu) for 16-bit types where a
 // KV head has rows enough and there are 8 chunks for each of its CTAs.  F16 takes
 // more rows: K and the weights go into that form in two parts.  Measured, that form
-// against this one (32 query over 8 KV heads, Q8_0, 8 sequences of up to 8000
-// positions): BF16 of 128 values, 48 rows 75 against 71 us, 56 rows 76 against 78,
-// 256 rows 112 against 260; of 64 values, 64 rows 57 against 55, 128 rows 61 against
-// 90; F16 of 128, 80 rows 100 against 94, 96 rows 102 against 116, 256 rows 155
-// against 260; of 64, 96 rows 72 against 70, 128 rows 75 against 89.  With fewer
-// chunks (BF16, 2 sequences of 8000, 128 rows, 2000 chunks) 73 against 56 us; one
-// sequence of 2000 positions, 256 rows, 39 against 29.
+// against this one (32 query over 8 KV heads, Q8_0, 8 sequences of 2700 to 8000
+// positions): BF16 of 128 values, 32 rows 66 against 56 us, 48 rows 68 against 75,
+// 56 rows 69 against 100, 256 rows 102 against 343; of 64 values, 48 rows 54
+// against 50, 64 rows 56 against 62, 128 rows 58 against 114; F16 of 128, 56 rows 85
+// against 99, 80 rows 88 against 119, 96 rows 89 against 139; of 64, 64 rows 64
+// against 62, 80 rows 65 against 75, 128 rows 66 against 114.  So it is ahead from one
+// or two tiles of 16 rows below the borders; they lie where they do since it also
+// rounds cached values to f16, which this one takes exactly.  With fewer chunks (BF16, 2
+// sequences of 8000, 128 rows, 2000 chunks) 69 against 58 us, with 3000 63 against 80;
+// one sequence of 2000 positions, 256 rows, 29 against 28.
 constexpr uint64_t kUmmaChunks = 8 * 296;
 bool can_use_umma(const m3g_kv_layout* l, uint32_t dtype, uint32_t n_heads, uint32_t max_tokens) {
   const uint64_t least = dtype == M3G_DTYPE_F16 ? 81 : l->head_dim == 128 ? 49 : 65;

@@ -27,13 +27,16 @@
 // overlap the other's softmax): a warpgroup for the softmax; one that unpacks K
 // and one that unpacks V, each warp 16 positions of the chunk; and four warps
 // that only issue: the scores, the results, and the bulk copies that bring K's
-// and V's codes and scales (rows of a page are contiguous) two chunks ahead.
+// and V's codes and scales (rows of a page are contiguous) two chunks ahead (F16
+// over Q8_0 with 128 values has room for one stage: there a copy starts when the chunk
+// before it is unpacked).
 // Measured: 8 trees of up to 64 tokens over contexts of up to 8190 (256 rows a KV
-// head, BF16 over Q8_0) 114 us, 12 trees of 13 over contexts of up to 30011 (104 rows,
-// F16 over Q4_0) 333 us.  Neither HBM nor the products bound it (their floors are
-// 21 and 44 us): a chunk takes a CTA 3300 cycles of softmax and unpacking in
-// turn, a piece some 13000 to start, and waiting for instructions costs as much
-// as any other stall.
+// head, BF16 over Q8_0) 100 us, 12 trees of 13 over contexts of up to 30011 (104 rows,
+// F16 over Q4_0) 280 us.  Neither HBM nor the products bound it (their floors are
+// 21 and 44 us): a chunk's softmax and unpacking follow one another, issue slots are
+// 60 % used, and waits for tensor memory, barriers and instructions share the rest.
+// Polls that hold a waiting thread for 2 us at most are part of that: with the
+// hardware's own limit the two cases took 114 and 333 us.
 // Scores run one chunk ahead of the weights.  Every role's chain of waits,
 // fences and issues is some 1000 cycles a chunk, so each has warps of its own: a
 // clock64 trace showed 5100 cycles a chunk with one issuing thread for both
