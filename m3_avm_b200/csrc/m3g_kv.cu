@@ -17,8 +17,8 @@
 // token each.
 //
 // Measured: 20954 BF16 tokens of 8 + 8 heads of 128 (5 ragged prompts) to Q4_0, written
-// 38.7 us (110 MB, 2.8 TB/s), read back 24.2 us (4.5 TB/s); 23918 tokens to Q8_0
-// 34.2 us (150 MB, 4.4 TB/s) and back 32.4 us (4.6 TB/s).  Issue slots are 70 % used
+// 39.2 us (110 MB, 2.8 TB/s), read back 24.5 us (4.5 TB/s); 23918 tokens to Q8_0
+// 34.8 us (150 MB, 4.3 TB/s) and back 33.0 us (4.6 TB/s).  Issue slots are 70 % used
 // in writing (125 instructions for a thread's 8 values to Q8_0, 167 to Q4_0, where 29 %
 // of the warps hold a value near a border), 64 % in reading (87).
 #include <algorithm>
@@ -179,18 +179,22 @@ __device__ __forceinline__ void find_places(const KvIoArgs& a, int t0, int n_tok
   __syncthreads();
 }
 
-// The starts into shared memory; the first CTA reports sequences outside the call's
-// limits, also those that no token leads to.
+// The starts into shared memory, where they fit.  The first CTA (all, where they
+// do not) looks the sequences over and reports those outside the call's limits,
+// also ones that no token leads to.
 __device__ __forceinline__ void hold_starts(const KvIoArgs& a, int32_t* starts) {
-  const int n_seqs = static_cast<int>(a.b.n_seqs);
+  const int n_seqs = static_cast<int>(a.b.n_seqs), tid = threadIdx.x;
   bool bad = false;
-  if (blockIdx.x == 0) {
-    for (int s = threadIdx.x; s < n_seqs; s += kKvThreads) {
+  if (n_seqs > kKvStarts) {
+    for (long long s = static_cast<long long>(blockIdx.x) * kKvThreads + tid; s < n_seqs; s += gridDim.x * kKvThreads)
+      seq_view(a.b, a.cap, static_cast<int>(s), &bad);
+  } else if (blockIdx.x == 0) {
+    for (int s = tid; s < n_seqs; s += kKvThreads) {
       const SeqView v = seq_view(a.b, a.cap, s, &bad);
-      if (n_seqs <= kKvStarts) starts[s] = v.q0;
+      starts[s] = v.q0;
     }
-  } else if (n_seqs <= kKvStarts) {
-    for (int s = threadIdx.x; s < n_seqs; s += kKvThreads) starts[s] = a.b.q_start[s];
+  } else {
+    for (int s = tid; s < n_seqs; s += kKvThreads) starts[s] = a.b.q_start[s];
   }
   if (bad) atomicOr(a.p.status, kStatusBadBatch);
   __syncthreads();

@@ -364,6 +364,36 @@ def test_every_operator_reports_every_bad_sequence(q_start, ctx):
     assert torch.equal(k[last].cpu(), R.quantised(x[last], True))
 
 
+@pytest.mark.parametrize("n", [300, 1024, 1025, 5000])
+def test_cache_of_many_sequences(n):
+    """More sequences than a CTA has threads, or starts in shared memory; one bad one anywhere is skipped and reported."""
+    from m3_avm_b200.attention import KvBatch, KvCache
+
+    r = np.random.default_rng(n)
+    ctx, new = [int(x) for x in r.integers(0, 40, n)], [int(x) for x in r.integers(0, 3, n)]
+    new[n - 2] = 2
+    batch, pages, table, start = R.make_batch(ctx, new, 16, seed=n)
+    cache = KvCache(8, 1, 1, 64, 16, pages)
+    x = randn(1, sum(new), 1, 64)
+    want = R.quantised(x, True)
+    for bad in (None, n - 2, 0):
+        cache.pool.zero_()
+        b = batch
+        if bad is not None:
+            wrong = torch.tensor(ctx, dtype=torch.int32)
+            wrong[bad] = -5
+            b = KvBatch(batch.q_start, wrong.cuda(), batch.page_table, batch.n_tokens, batch.max_tokens, batch.max_len)
+        cache.write(0, x, x, b)
+        assert status() == (0 if bad is None else 16)
+        k = torch.full_like(x, 7.0)
+        cache.read(0, b, k_out=k, v_out=torch.empty_like(x))
+        assert status() == (0 if bad is None else 16)
+        skipped = torch.zeros(sum(new), dtype=torch.bool)
+        if bad is not None:
+            skipped[int(start[bad]):int(start[bad + 1])] = True
+        assert torch.equal(k.cpu()[~skipped], want[~skipped]) and bool((k.cpu()[skipped] == 7).all())
+
+
 @pytest.mark.parametrize("dtype,heads,large", [(F32, 4, False), (BF16, 4, False), (F16, 4, False), (BF16, 64, True),
                                                (F16, 64, True)])
 @pytest.mark.parametrize("at", [3, 41])
