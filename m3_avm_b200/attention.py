@@ -133,13 +133,16 @@ def _check_ints(name, t, device, shape):
 
 
 class _Told:
-    """What the library was told once, by value and by address: public attributes stay as they were made.  (A changed
-    n_tokens would pass the checks of the tensors here, and the kernels would still go by the old one.)"""
+    """What the library was told once, by value and by address: the attributes made here stay.  (A changed n_tokens
+    would pass the checks of the tensors, and the kernels would still go by the old one.)"""
 
-    _done = False
+    _told = frozenset()
+
+    def _seal(self):
+        self._told = frozenset(name for name in self.__dict__ if not name.startswith("_"))
 
     def __setattr__(self, name, value):
-        if self._done and not name.startswith("_"):
+        if name in self._told:
             _fail(f"{type(self).__name__}.{name} cannot be changed: make a new {type(self).__name__}")
         object.__setattr__(self, name, value)
 
@@ -162,7 +165,7 @@ class Rope(_Told):
         h = ctypes.c_void_p()
         _lib.check(_lib.load().m3g_rope_create(ctypes.byref(cfg), ctypes.byref(h)))
         self._h = h
-        self._done = True
+        self._seal()
 
     def apply(self, positions, q, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
         """Turns q and k (k may be None) at int32 `positions` (tokens,); q_out, k_out may be q and k themselves.
@@ -220,7 +223,7 @@ class KvBatch(_Told):
         self.n_tokens, self.max_tokens, self.max_len = n_tokens, max_tokens, max_len
         self.args = _lib.KvBatchArgs(q_start.data_ptr(), ctx_len.data_ptr(), page_table.data_ptr(), n,
                                      page_table.shape[1], n_tokens, max_tokens, max_len)
-        self._done = True
+        self._seal()
 
 
 class KvCache(_Told):
@@ -244,7 +247,7 @@ class KvCache(_Told):
         self.pool = pool
         self.device = pool.get_device()
         self._workspace_bytes: dict[tuple, int] = {}
-        self._done = True
+        self._seal()
 
     def _check_layer(self, layer):
         if not 0 <= layer < self.n_layers:  # here: the library would get its low 32 bits

@@ -178,4 +178,14 @@ def test_what_the_library_was_told_cannot_be_changed_behind_its_back():
             setattr(obj, name, value)
         assert getattr(obj, name) is before
     batch.ctx_len[0] = 7  # the contents are the caller's
+
+    class Mine(A.KvCache):  # and so are attributes of their own
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            self.free = [1]
+
+    mine = Mine(8, 1, 2, 64, 16, 4, pool=cache.pool)
+    mine.free = []
+    with pytest.raises(M3GError, match="cannot be changed"):
+        mine.head_dim = 128
     rope.close()
